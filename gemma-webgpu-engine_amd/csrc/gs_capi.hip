@@ -54,6 +54,12 @@ struct gs_context {
   uint64_t* d_plists = nullptr;
   uint32_t* d_row_thr = nullptr;
   int32_t fused_rows = 0;
+  // work memory of the loss and of the gradients (grown on demand). A block
+  // that was outgrown is kept until the context ends: a captured graph may
+  // hold its address.
+  uint8_t* d_work = nullptr;
+  size_t work_cap = 0;
+  std::vector<void*> old_work;
   // kernel timing (gs_timing_begin / gs_timing_end): per timed call and stage,
   // the start and stop events of that stage's kernel launch
   std::vector<hipEvent_t> t_events;  // [max_calls][GS_STAGE_COUNT][2]
@@ -165,6 +171,37 @@ int ensure_fused(gs_context* ctx, int32_t rows) {
     return fail(ctx, GS_ERR_HIP, "allocating the fused lm_head buffers failed");
   }
   ctx->fused_rows = (int32_t)r;
+  return GS_OK;
+}
+
+// The calling thread's current device, put back at the end of a call.
+struct DeviceGuard {
+  int before = -1;
+  DeviceGuard() {
+    if (hipGetDevice(&before) != hipSuccess) before = -1;
+  }
+  ~DeviceGuard() {
+    if (before >= 0) (void)hipSetDevice(before);
+  }
+};
+
+// Grows the context's work memory to at least `bytes`, by a quarter more than
+// asked once there is some. Nothing waits: queued work keeps the old block.
+int ensure_work(gs_context* ctx, size_t bytes, hipStream_t s) {
+  if (bytes <= ctx->work_cap) return GS_OK;
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  GS_HIP(ctx, hipStreamIsCapturing(s, &capture));
+  if (capture != hipStreamCaptureStatusNone)
+    return fail(ctx, GS_ERR_UNSUPPORTED, "the work memory cannot grow under capture: make the call once before it");
+  const size_t want = ctx->work_cap ? bytes + bytes / 4 : bytes;
+  uint8_t* p = nullptr;
+  if (hipMalloc(&p, want) != hipSuccess) {
+    (void)hipGetLastError();
+    return fail(ctx, GS_ERR_HIP, "allocating the work memory failed");
+  }
+  if (ctx->d_work) ctx->old_work.push_back(ctx->d_work);
+  ctx->d_work = p;
+  ctx->work_cap = want;
   return GS_OK;
 }
 
@@ -322,6 +359,41 @@ Workspace context_workspace(const gs_context* ctx) {
   w.deep_queue = ctx->d_deep_queue;
   w.deep_max_rows = ctx->max_rows;
   return w;
+}
+
+constexpr int64_t kMxMaxValues = (int64_t)1 << 34;  // 8 a thread: a launch holds less than 2^32 threads
+constexpr int32_t kMxHeadMaxWidth = 16384;
+constexpr int32_t kHeadMaxRows = 1 << 20;
+constexpr int64_t kMaxTiles = (int64_t)1 << 22;  // of 512 threads, for the same reason
+
+// The first thing wrong with a norm's sizes and types (NULL: nothing).
+const char* norm_error(gs_context* ctx, int32_t dtype, int32_t weight_dtype, int32_t rows, int32_t width, float eps,
+                       float offset) {
+  if (!ctx || rows < 0 || width <= 0) return "bad arguments";
+  if ((dtype != GS_F32 && dtype != GS_BF16) || (weight_dtype != GS_F32 && weight_dtype != GS_BF16))
+    return "dtype must be f32 or bf16";
+  if (!(eps >= 0) || !std::isfinite(eps) || !std::isfinite(offset)) return "eps must be >= 0, and weight_offset finite";
+  return nullptr;
+}
+
+const char* mx_error(gs_context* ctx, int32_t dtype, int32_t format, int64_t rows, int32_t width) {
+  if (!ctx || rows < 0 || width <= 0) return "bad arguments";
+  if (dtype != GS_F32 && dtype != GS_BF16) return "dtype must be f32 or bf16";
+  if (format != GS_MX_E2M1 && format != GS_MX_E4M3) return "format must be e2m1 or e4m3";
+  return nullptr;
+}
+
+// The sizes of a loss call. The kernels address H, a piece of W and a piece of
+// the gradients with 31-bit byte offsets.
+int loss_check(gs_context* ctx, int32_t rows, int32_t width) {
+  if (!ctx || rows < 0 || width <= 0) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "bad arguments");
+  if (width % 64 != 0 || width > 65536)
+    return fail(ctx, GS_ERR_UNSUPPORTED, "lm_head width must be a multiple of 64, at most 65536");
+  if (rows > kHeadMaxRows || (int64_t)rows * width >= ((int64_t)1 << 30))
+    return fail(ctx, GS_ERR_UNSUPPORTED, "at most 1048576 rows and 2^30 hidden values a call");
+  if ((int64_t)((ctx->vocab + 255) / 256) * ((rows + 63) / 64) > kMaxTiles)
+    return fail(ctx, GS_ERR_UNSUPPORTED, "too many logits in one call");
+  return GS_OK;
 }
 
 void destroy_timing(gs_context* ctx) {
@@ -514,6 +586,8 @@ int gs_destroy(gs_context* ctx) {
   free_dev(ctx->d_parts);
   free_dev(ctx->d_plists);
   free_dev(ctx->d_row_thr);
+  free_dev(ctx->d_work);
+  for (void* p : ctx->old_work) free_dev(p);
   destroy_timing(ctx);
   if (ctx->stream) (void)hipStreamDestroy(ctx->stream);
   delete ctx;
@@ -1089,6 +1163,221 @@ int gs_lmhead_sample(gs_context* ctx, const void* hidden, const void* weight, in
   if (e == hipSuccess) e = launch_sample(w, &b, s, ev, &f);
   if (e != hipSuccess) return fail(ctx, GS_ERR_HIP, std::string("kernel launch: ") + hipGetErrorString(e));
   if (slot >= 0) ctx->t_calls++;
+  return GS_OK;
+}
+
+int gs_rms_norm(gs_context* ctx, const void* x, const void* residual, const void* weight, int32_t dtype,
+                int32_t weight_dtype, int32_t rows, int32_t width, int64_t x_stride, int64_t residual_stride,
+                float eps, float weight_offset, void* summed, void* out, uint8_t* codes, uint8_t* scales, void* stream) {
+  const char* bad = norm_error(ctx, dtype, weight_dtype, rows, width, eps, weight_offset);
+  if (!bad && (!codes != !scales)) bad = "codes and scales go together";
+  if (!bad && rows && !summed && !out && !codes) bad = "no output is given";
+  if (bad) return fail(ctx, GS_ERR_INVALID_ARGUMENT, bad);
+  if (width > kNormMaxWidth) return fail(ctx, GS_ERR_UNSUPPORTED, "rms_norm width must be at most 16384");
+  if (codes && width % 32 != 0) return fail(ctx, GS_ERR_UNSUPPORTED, "e4m3 blocks need a width that is a multiple of 32");
+  if (rows == 0) return GS_OK;
+  if (!x || !weight) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "x and weight are required");
+  if ((rows > 1 && x_stride < width) || (residual && rows > 1 && residual_stride < width))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "a row stride is smaller than the width");
+  const uintptr_t mask = dtype == GS_BF16 ? 1 : 3;
+  if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)summed | (uintptr_t)out) & mask ||
+      ((uintptr_t)weight & (weight_dtype == GS_BF16 ? 1 : 3)))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
+  if (codes && !aligned16(codes)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned");
+  DeviceGuard guard;
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  NormArgs a{};
+  a.x = x;
+  a.residual = residual;
+  a.weight = weight;
+  a.summed = summed;
+  a.out = out;
+  a.codes = codes;
+  a.scales = scales;
+  a.x_stride = rows > 1 ? x_stride : 0;
+  a.residual_stride = rows > 1 ? residual_stride : 0;
+  a.rows = rows;
+  a.width = width;
+  a.weight_bf16 = weight_dtype == GS_BF16;
+  a.eps = eps;
+  a.offset = weight_offset;
+  launch_rms_norm(a, dtype == GS_BF16, pick_stream(ctx, stream));
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_rms_norm_grad(gs_context* ctx, const void* dy, const void* h, const void* weight, const void* dsummed,
+                     int32_t dtype, int32_t weight_dtype, int32_t rows, int32_t width, int64_t dy_stride,
+                     int64_t h_stride, int64_t dsummed_stride, float eps, float weight_offset, void* dx,
+                     float* dweight, void* stream) {
+  const char* bad = norm_error(ctx, dtype, weight_dtype, rows, width, eps, weight_offset);
+  if (!bad && rows && !dx && !dweight) bad = "no output is given";
+  if (bad) return fail(ctx, GS_ERR_INVALID_ARGUMENT, bad);
+  if (width > kNormMaxWidth) return fail(ctx, GS_ERR_UNSUPPORTED, "rms_norm width must be at most 16384");
+  DeviceGuard guard;
+  hipStream_t s = pick_stream(ctx, stream);
+  if (rows == 0) {
+    if (!dweight) return GS_OK;
+    GS_HIP(ctx, hipSetDevice(ctx->device));
+    launch_fill_zero(dweight, (int64_t)width * 4, s);
+    GS_HIP(ctx, hipGetLastError());
+    return GS_OK;
+  }
+  if (!dy || !h || !weight) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "dy, h and weight are required");
+  if (rows > 1 && (dy_stride < width || h_stride < width || (dsummed && dsummed_stride < width)))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "a row stride is smaller than the width");
+  const uintptr_t mask = dtype == GS_BF16 ? 1 : 3;
+  if (((uintptr_t)dy | (uintptr_t)h | (uintptr_t)dsummed | (uintptr_t)dx) & mask ||
+      ((uintptr_t)weight & (weight_dtype == GS_BF16 ? 1 : 3)) || ((uintptr_t)dweight & 3))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  if (dweight) {
+    const int st = ensure_work(ctx, (size_t)norm_parts(rows, width) * width * sizeof(float), s);
+    if (st != GS_OK) return st;
+  }
+  NormGradArgs a{};
+  a.dy = dy;
+  a.h = h;
+  a.weight = weight;
+  a.dsummed = dsummed;
+  a.dx = dx;
+  a.parts = dweight ? (float*)ctx->d_work : nullptr;
+  a.dy_stride = rows > 1 ? dy_stride : 0;
+  a.h_stride = rows > 1 ? h_stride : 0;
+  a.dsummed_stride = rows > 1 ? dsummed_stride : 0;
+  a.rows = rows;
+  a.width = width;
+  a.weight_bf16 = weight_dtype == GS_BF16;
+  a.eps = eps;
+  a.offset = weight_offset;
+  launch_rms_norm_grad(a, dtype == GS_BF16, dweight, s);
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_mx_quantize(gs_context* ctx, const void* x, int32_t dtype, int32_t format, int64_t rows, int32_t width,
+                   int64_t row_stride, uint8_t* codes, uint8_t* scales, void* stream) {
+  const char* bad = mx_error(ctx, dtype, format, rows, width);
+  if (bad) return fail(ctx, GS_ERR_INVALID_ARGUMENT, bad);
+  if (width % 32 != 0) return fail(ctx, GS_ERR_UNSUPPORTED, "microscaled rows need a width that is a multiple of 32");
+  if (rows > kMxMaxValues / width) return fail(ctx, GS_ERR_UNSUPPORTED, "too many values in one call");
+  if (rows == 0) return GS_OK;
+  if (!x || !codes || !scales) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "x, codes and scales are required");
+  if (rows > 1 && row_stride < width) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "row_stride is smaller than the width");
+  if (((uintptr_t)x & (dtype == GS_BF16 ? 1 : 3)) || !aligned16(codes))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "x must be aligned to its elements, codes to 16 bytes");
+  DeviceGuard guard;
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  launch_mx_quantize(x, dtype == GS_BF16, format, rows, width, row_stride, codes, scales, pick_stream(ctx, stream));
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_mx_dequantize(gs_context* ctx, const uint8_t* codes, const uint8_t* scales, int32_t format, int64_t rows,
+                     int32_t width, int32_t dtype, void* out, void* stream) {
+  const char* bad = mx_error(ctx, dtype, format, rows, width);
+  if (bad) return fail(ctx, GS_ERR_INVALID_ARGUMENT, bad);
+  if (width % 32 != 0) return fail(ctx, GS_ERR_UNSUPPORTED, "microscaled rows need a width that is a multiple of 32");
+  if (rows > kMxMaxValues / width) return fail(ctx, GS_ERR_UNSUPPORTED, "too many values in one call");
+  if (rows == 0) return GS_OK;
+  if (!codes || !scales || !out) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes, scales and out are required");
+  if (!aligned16(codes) || !aligned16(out)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes and out must be 16-byte aligned");
+  DeviceGuard guard;
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  launch_mx_dequantize(codes, scales, format, rows, width, dtype == GS_BF16, out, pick_stream(ctx, stream));
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
+                 const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t m_rows, int32_t width,
+                 float softcap, float* logits, void* stream) {
+  if (!ctx || m_rows < 0 || width <= 0) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "bad arguments");
+  if (width % 64 != 0 || width > kMxHeadMaxWidth)
+    return fail(ctx, GS_ERR_UNSUPPORTED, "microscaled lm_head width must be a multiple of 64, at most 16384");
+  if (m_rows > kHeadMaxRows || (int64_t)(ctx->vocab / 256 + 8) * ((m_rows + 127) / 128) > kMaxTiles)
+    return fail(ctx, GS_ERR_UNSUPPORTED, "too many logits in one call");
+  if (m_rows == 0) return GS_OK;
+  if (!hidden_codes || !hidden_scales || !weight_codes || !weight_scales || !logits)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes, scales and logits are required");
+  if (!aligned16(hidden_codes) || !aligned16(weight_codes))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned");
+  if (((uintptr_t)hidden_scales | (uintptr_t)weight_scales) & 1)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "scales must be 2-byte aligned");
+  if ((uintptr_t)logits & 3) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "logits must be aligned to their elements");
+  DeviceGuard guard;
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  const int32_t slot = timing_slot(ctx);
+  launch_mx_lmhead(hidden_codes, hidden_scales, weight_codes, weight_scales, m_rows, width, ctx->vocab, softcap, logits,
+                   pick_stream(ctx, stream), stage_events(ctx, slot, GS_STAGE_LMHEAD));
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_mx_lmhead_sample(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
+                        const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t width, float softcap,
+                        float* logits_scratch, const gs_batch* batch, void* stream) {
+  if (!batch) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "bad arguments");
+  int st = gs_mx_lmhead(ctx, hidden_codes, hidden_scales, weight_codes, weight_scales, batch->rows, width, softcap,
+                        logits_scratch, stream);
+  if (st != GS_OK) return st;
+  gs_batch b = *batch;
+  b.logits = logits_scratch;
+  b.dtype = GS_F32;
+  b.row_stride = ctx->vocab;
+  return gs_sample(ctx, &b, stream);
+}
+
+int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets, int32_t rows,
+                   int32_t width, float softcap, float* loss, float* lse, void* stream) {
+  int st = loss_check(ctx, rows, width);
+  if (st != GS_OK || rows == 0) return st;
+  if (!hidden || !weight || !targets || !loss || !lse)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden, weight, targets, loss and lse are required");
+  if (!aligned16(hidden) || !aligned16(weight)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden and weight must be 16-byte aligned");
+  if (((uintptr_t)targets | (uintptr_t)loss | (uintptr_t)lse) & 3)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "targets, loss and lse must be aligned to their elements");
+  DeviceGuard guard;
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  hipStream_t s = pick_stream(ctx, stream);
+  const LossPlan plan = loss_plan(rows, width, ctx->vocab, ctx->cu_count);
+  st = ensure_work(ctx, plan.stats_bytes, s);
+  if (st != GS_OK) return st;
+  launch_lmhead_loss((const uint16_t*)hidden, (const uint16_t*)weight, targets, rows, width, ctx->vocab, softcap, plan,
+                     ctx->d_work, loss, lse, s);
+  GS_HIP(ctx, hipGetLastError());
+  return GS_OK;
+}
+
+int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets,
+                        const float* lse, const float* dloss, int32_t rows, int32_t width, float softcap,
+                        void* dhidden, void* dweight, void* stream) {
+  int st = loss_check(ctx, rows, width);
+  if (st != GS_OK) return st;
+  if (rows && !dhidden && !dweight) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "no output is given");
+  if (!aligned16(dhidden) || !aligned16(dweight))
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "dhidden and dweight must be 16-byte aligned");
+  DeviceGuard guard;
+  hipStream_t s = pick_stream(ctx, stream);
+  if (rows == 0) {
+    if (!dweight) return GS_OK;
+    GS_HIP(ctx, hipSetDevice(ctx->device));
+    launch_fill_zero(dweight, (int64_t)ctx->vocab * width * 2, s);
+    GS_HIP(ctx, hipGetLastError());
+    return GS_OK;
+  }
+  if (!hidden || !weight || !targets || !lse || !dloss)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden, weight, targets, lse and dloss are required");
+  if (!aligned16(hidden) || !aligned16(weight)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden and weight must be 16-byte aligned");
+  if (((uintptr_t)targets | (uintptr_t)lse | (uintptr_t)dloss) & 3)
+    return fail(ctx, GS_ERR_INVALID_ARGUMENT, "targets, lse and dloss must be aligned to their elements");
+  GS_HIP(ctx, hipSetDevice(ctx->device));
+  const LossPlan plan = loss_plan(rows, width, ctx->vocab, ctx->cu_count);
+  st = ensure_work(ctx, plan.g_bytes + plan.h_bytes + plan.part_bytes, s);
+  if (st != GS_OK) return st;
+  launch_lmhead_loss_grad((const uint16_t*)hidden, (const uint16_t*)weight, targets, lse, dloss, rows, width, ctx->vocab,
+                          softcap, plan, ctx->d_work, (uint16_t*)dhidden, (uint16_t*)dweight, s);
+  GS_HIP(ctx, hipGetLastError());
   return GS_OK;
 }
 

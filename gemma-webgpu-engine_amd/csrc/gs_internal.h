@@ -615,4 +615,65 @@ void launch_lmhead_scan(const uint16_t* hidden, const uint16_t* weight, int32_t 
                         float* out, const SampleArgs& a, const FusedArgs& f, hipStream_t s, LaunchEvents ev = {});
 void launch_merge_parts(const SampleArgs& a, const FusedArgs& f, hipStream_t s, LaunchEvents ev = {});
 
+// ------------------------------------------- the norm before the head
+constexpr int32_t kNormMaxWidth = 16384;  // a row is held in one workgroup's registers
+struct NormArgs {
+  const void* x;
+  const void* residual;  // NULL: none
+  const void* weight;
+  void* summed;          // NULL: not written
+  void* out;             // NULL: not written
+  uint8_t* codes;        // NULL: no e4m3 blocks
+  uint8_t* scales;
+  int64_t x_stride, residual_stride;  // elements
+  int32_t rows, width, weight_bf16;
+  float eps, offset;
+};
+struct NormGradArgs {
+  const void* dy;
+  const void* h;
+  const void* weight;
+  const void* dsummed;  // NULL: none
+  void* dx;             // NULL: not written
+  float* parts;         // [norm_parts][width] shares of dweight; NULL: not wanted
+  int64_t dy_stride, h_stride, dsummed_stride;
+  int32_t rows, width, weight_bf16;
+  float eps, offset;
+};
+bool norm_wave_rows(int32_t rows, int32_t width);
+int32_t norm_parts(int32_t rows, int32_t width);
+void launch_rms_norm(const NormArgs& a, bool bf16, hipStream_t s);
+void launch_rms_norm_grad(const NormGradArgs& a, bool bf16, float* dweight, hipStream_t s);
+
+// `bytes` (a multiple of 2) zeros, by a kernel: capturable anywhere.
+void launch_fill_zero(void* p, int64_t bytes, hipStream_t s);
+
+// ------------------------------------------- microscaled blocks and the 4-bit head
+void launch_mx_quantize(const void* x, bool bf16, int32_t format, int64_t rows, int32_t width, int64_t row_stride,
+                        uint8_t* codes, uint8_t* scales, hipStream_t s);
+void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int32_t format, int64_t rows, int32_t width,
+                          bool bf16, void* out, hipStream_t s);
+void launch_mx_lmhead(const uint8_t* hidden, const uint8_t* hidden_scales, const uint8_t* weight,
+                      const uint8_t* weight_scales, int32_t m, int32_t width, int32_t vocab, float softcap, float* out,
+                      hipStream_t s, LaunchEvents ev = {});
+
+// ------------------------------------------- the head's cross entropy
+struct LossPlan {
+  int32_t cols;        // rows of H in a tile: 64, 128 or 256
+  int32_t v_tiles;     // tiles of 256 vocabulary rows
+  int32_t piece;       // vocabulary rows whose gradients are held at a time, a multiple of 256
+  int32_t splits;      // shares of a piece's vocabulary in dhidden's product
+  size_t stats_bytes;  // forward: a (max, sum) per row and tile
+  size_t g_bytes;      // backward: a piece's gradients of the logits in bf16
+  size_t h_bytes;      // backward: H with the rows that are not scored set to zero
+  size_t part_bytes;   // backward: dhidden's shares
+};
+LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count);
+void launch_lmhead_loss(const uint16_t* hidden, const uint16_t* weight, const int32_t* targets, int32_t rows,
+                        int32_t width, int32_t vocab, float softcap, const LossPlan& plan, uint8_t* work, float* loss,
+                        float* lse, hipStream_t s);
+void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, const int32_t* targets, const float* lse,
+                             const float* dloss, int32_t rows, int32_t width, int32_t vocab, float softcap,
+                             const LossPlan& plan, uint8_t* work, uint16_t* dhidden, uint16_t* dweight, hipStream_t s);
+
 }  // namespace gs

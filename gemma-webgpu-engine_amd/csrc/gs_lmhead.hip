@@ -19,7 +19,7 @@
 // What bounds the GEMM: memory up to about 160 rows; past that the operand
 // traffic of the tiles (12 TB/s from the L2s at M 512), the matrix cores 42%
 // busy. The totals of the ranges take the registers that a larger tile would.
-#include "gs_internal.h"
+#include "gs_cap.h"
 
 namespace gs {
 namespace {
@@ -33,51 +33,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 // any time over the channels (M 128, D 2048, V 262144: 265 us with one start
 // for all, 230 so; widths off such strides measure the same either way).
 __device__ __forceinline__ int lmhead_first_range(int64_t v, int D) { return D % 512 == 0 ? (int)((v >> 7) & 7) : 0; }
-
-// cap tanh(x / cap) of kN values of each lane. Below 5/8 tanh q is
-// q + q^3 P(q^2), P of degree 5 fitted over that range (relative error of the
-// fit 2^-32; at most 0.70 ulp with its roundings); a wave whose values all lie
-// there evaluates them side by side, where a tanhf a value, each behind its
-// own branch, was one long chain (60 of 690 us at M 512, D 2048, V 262144).
-// Their x / cap rounded to nearest takes two fused multiply-adds from
-// r = 1 / cap rounded to nearest (Markstein: the remainder of q0 = x r is
-// exact, and its share r completes the quotient). Every value takes the same
-// formula in either branch. r = 0 (cap outside 2^+-60): always the division.
-constexpr float kTanhSmall = 0.625f;
-__device__ __forceinline__ float tanh_small(float q) {
-  const float s = q * q;
-  float p = 0x1.197b58p-9f;
-  p = __builtin_fmaf(p, s, -0x1.0c213cp-7f);
-  p = __builtin_fmaf(p, s, 0x1.6394d6p-6f);
-  p = __builtin_fmaf(p, s, -0x1.b9ef7cp-5f);
-  p = __builtin_fmaf(p, s, 0x1.11106cp-3f);
-  p = __builtin_fmaf(p, s, -0x1.555554p-2f);
-  return __builtin_fmaf(q * s, p, q);
-}
-__device__ __forceinline__ float reciprocal_of_cap(float cap) {
-  return cap >= 0x1p-60f && cap <= 0x1p60f ? 1.0f / cap : 0.0f;
-}
-template <int kN>
-__device__ __forceinline__ void lmhead_cap(float (&x)[kN], float cap, float r) {
-  float q[kN];
-  bool small = r != 0.0f;
-#pragma unroll
-  for (int e = 0; e < kN; ++e) {
-    const float q0 = x[e] * r;
-    q[e] = __builtin_fmaf(__builtin_fmaf(-q0, cap, x[e]), r, q0);
-    small = small && __builtin_fabsf(q[e]) < kTanhSmall;  // (false for a NaN)
-  }
-  if (__all(small)) {
-#pragma unroll
-    for (int e = 0; e < kN; ++e) x[e] = cap * tanh_small(q[e]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kN; ++e) {
-      const float v = x[e] / cap;
-      x[e] = cap * (__builtin_fabsf(v) < kTanhSmall ? tanh_small(v) : tanhf(v));
-    }
-  }
-}
 
 constexpr int kGemmThreads = 256;  // 2 x 2 waves over (V, M)
 constexpr int kGemmK = 64;         // K block: one 128-byte line of every row

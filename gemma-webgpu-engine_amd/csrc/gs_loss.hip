@@ -1,0 +1,635 @@
+// Softmax cross entropy of the head's logits, and its gradients, without the
+// logits in memory:
+//   z = cap(H W^T),  lse[m] = log sum_v exp z[m][v],  loss[m] = lse[m] - z[m][t[m]]
+//   g[m][v] = dloss[m] (exp(z[m][v] - lse[m]) - [v = t[m]]) (1 - (z[m][v] / cap)^2)
+//   dH = g W,  dW = g^T H
+//
+// Four products on v_mfma_f32_16x16x32_bf16 with one main loop (tiles of 256
+// rows by kCols columns, 8 waves, 64 of the summed index a stage, operands by
+// the memory pipe straight into LDS):
+//   kStats   W x H, the epilogue leaves a (max, sum) per hidden row and tile;
+//   kGrad    W x H again, a piece of the vocabulary, the epilogue writes g in
+//            bf16 (the matrix cores read 16 bits: half a step of 2^-9 a value,
+//            sums in binary32);
+//   kHidden  W^T x g, summed over the piece, in shares of its vocabulary rows;
+//   kWeight  H^T x g^T, summed over the hidden rows.
+// kHidden and kWeight sum over an operand's rows: those tiles lie in LDS as
+// they do in memory and are transposed by the LDS reads (ds_read_b64_tr_b16).
+#include <algorithm>
+
+#include "gs_cap.h"
+#include "gs_mx.h"
+
+namespace gs {
+namespace {
+
+enum Pass { kStats, kGrad, kHidden, kWeight };
+
+constexpr int kLossThreads = 512;
+constexpr int kRows = 256;  // rows of a tile (vocabulary rows; columns of K in kHidden and kWeight)
+constexpr int kBlock = 64;  // of the summed index a stage
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kLowest = -1.0e38f;  // a maximum over nothing; times log2(e) still finite
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef short i16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) void* LdsPtr;
+typedef __attribute__((address_space(3))) i16x4* LdsTrPtr;
+
+struct LossArgs {
+  const uint16_t* W;   // the piece's first row
+  const uint16_t* H;
+  uint16_t* G;         // [M][g_stride]
+  const int32_t* targets;
+  const float* lse;
+  const float* dloss;
+  float2* stats;       // kStats: [v_tiles][M]
+  float* part;         // kHidden: [splits][M][D]
+  uint16_t* dW;        // kWeight: the piece's first row
+  float cap;
+  int32_t M, D, V;     // V: vocabulary rows of the piece
+  int32_t v_base;      // the piece's first vocabulary row
+  int32_t vocab;
+  int32_t g_stride;    // a multiple of 256, at least V
+  int32_t row_tiles, col_tiles, splits, split_rows;  // split_rows: vocabulary rows a share, a multiple of 64
+  int32_t accumulate;  // kHidden: add to the shares of the pieces before
+};
+
+template <Pass kPass, int kCols>
+struct Tile {
+  static constexpr bool kTrA = kPass == kHidden || kPass == kWeight, kTrB = kPass == kWeight;
+  static constexpr int kWavesR = kCols == 256 ? 2 : kCols == 128 ? 4 : 8;
+  static constexpr int kWavesC = 8 / kWavesR;
+  static constexpr int kRT = 16 / kWavesR;          // 16-row tiles a wave
+  static constexpr int kCT = kCols / 16 / kWavesC;  // 16-column tiles a wave
+  static constexpr int kStages = kCols == 256 ? 2 : 3;
+  static constexpr int kA = kRows * kBlock * 2, kB = kCols * kBlock * 2;
+  static constexpr int kStage = kA + kB;
+  static constexpr int kFetchB = kCols / 64;
+  static constexpr int kFetches = 4 + kFetchB;
+  static constexpr int kOutStride = 256 + 8;        // 16-bit values a staged output row
+  static constexpr int kOut = kPass == kGrad || kPass == kWeight ? kCols * kOutStride * 2 : 0;
+  static constexpr int kLds = kStages * kStage > kOut ? kStages * kStage : kOut;
+  static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
+};
+
+// The position of 16-byte chunk pairs in a transposed tile's row: the 8 rows
+// that a half wave reads together (4 of each of two lane groups) take 8
+// different pairs of the banks.
+__device__ __forceinline__ int pair_swizzle(int row) { return (row & 3) | ((row >> 1) & 4); }
+
+// A stage's fetches of one operand: kN wave instructions of 1 KB. `tail`: bits
+// of lanes past the last summed row (transposed operands; uniform 0 elsewhere).
+template <int kN, typename Rsrc>
+__device__ __forceinline__ void loss_fetch(Rsrc r, char* lds, const uint32_t (&off)[kN], uint32_t k, uint32_t none) {
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * i), 16, off[i] | none, k, 0, 0);
+#endif
+}
+
+// Operand tile t's values of the summed index 32 s + 8 g .. + 7 for lane (j, g).
+template <bool kTr>
+__device__ __forceinline__ bf16x8 loss_operand(const char* p, int t, int s, uint32_t pos0, uint32_t pos1) {
+  if (!kTr) return *(const bf16x8*)(p + 2048 * t + (s ? pos1 : pos0));
+#ifdef __HIP_DEVICE_COMPILE__
+  // pos0: this lane's row and place in a pair, pos1: its swizzle
+  const char* q = p + s * 16384 + pos0 + ((32 * (uint32_t)t) ^ pos1);
+  const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTrPtr)q);
+  const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTrPtr)(q + 2048));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#else
+  return bf16x8{};
+#endif
+}
+
+template <Pass kPass, int kCols, typename Rsrc>
+__device__ __forceinline__ void loss_block(const char* __restrict__ a, const char* __restrict__ b,
+                                           char* __restrict__ a_next, char* __restrict__ b_next, Rsrc ar, Rsrc br,
+                                           const uint32_t (&a_off)[4],
+                                           const uint32_t (&b_off)[Tile<kPass, kCols>::kFetchB], uint32_t ak,
+                                           uint32_t bk, uint32_t a_none, uint32_t b_none, int a_tile, int b_tile,
+                                           const uint32_t (&a_pos)[2], const uint32_t (&b_pos)[2],
+                                           f32x4 (&acc)[Tile<kPass, kCols>::kRT][Tile<kPass, kCols>::kCT]) {
+  typedef Tile<kPass, kCols> T;
+  loss_fetch<4>(ar, a_next, a_off, ak, a_none);
+  loss_fetch<T::kFetchB>(br, b_next, b_off, bk, b_none);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    bf16x8 x[T::kRT], y[T::kCT];
+#pragma unroll
+    for (int i = 0; i < T::kRT; ++i) x[i] = loss_operand<T::kTrA>(a, a_tile + i, s, a_pos[0], a_pos[1]);
+#pragma unroll
+    for (int i = 0; i < T::kCT; ++i) y[i] = loss_operand<T::kTrB>(b, b_tile + i, s, b_pos[0], b_pos[1]);
+#pragma unroll
+    for (int i = 0; i < T::kRT; ++i) {
+#pragma unroll
+      for (int c = 0; c < T::kCT; ++c)
+        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[c], acc[i][c], 0, 0, 0);
+    }
+  }
+}
+
+// t = tanh(x / cap) of four values. Below 5/8 a polynomial (gs_cap.h), past it
+// 1 - 2 / (e^2q + 1): absolute errors near 1e-7 of the cap either way, which
+// the logarithm of the sum keeps.
+__device__ __forceinline__ void loss_tanh(const f32x4& x, float rcap, float (&t)[4]) {
+  float q[4];
+  bool small = true;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    q[e] = x[e] * rcap;
+    small = small && __builtin_fabsf(q[e]) < kTanhSmall;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) t[e] = tanh_small(q[e]);
+  if (!__all(small)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float w = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(q[e] * (2.0f * kLog2e)) + 1.0f);
+      if (!(__builtin_fabsf(q[e]) < kTanhSmall)) t[e] = w;
+    }
+  }
+}
+
+template <Pass kPass, int kCols>
+__global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
+  typedef Tile<kPass, kCols> T;
+  __shared__ __attribute__((aligned(16))) char lds[T::kLds];
+  // An XCD (consecutive workgroups go to them in turn) takes a run of adjacent
+  // tiles, so its workgroups share their operands' lines in its L2: four row
+  // tiles by all column tiles (kStats, kGrad), all row tiles by a run of
+  // column tiles (kHidden, kWeight).
+  const int total = p.row_tiles * p.col_tiles * p.splits;
+  int id = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
+  if (id >= total) return;
+  int rt, ct, split = 0;
+  if (kPass == kStats || kPass == kGrad) {
+    const int group = id / (4 * p.col_tiles) * 4;
+    const int in = p.row_tiles - group < 4 ? p.row_tiles - group : 4;
+    id -= group * p.col_tiles;
+    rt = group + id % in;
+    ct = id / in;
+  } else {
+    rt = id % p.row_tiles;
+    id /= p.row_tiles;
+    ct = id % p.col_tiles;
+    split = id / p.col_tiles;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4, wr = wave % T::kWavesR, wc = wave / T::kWavesR;
+  const int M = p.M, D = p.D, V = p.V;
+  const int r0 = rt * kRows, c0 = ct * kCols;
+
+  // operands: where their first row lies, how many rows there are, their stride
+  const int sum0 = kPass == kHidden ? split * p.split_rows : 0;  // first of the summed index
+  int sums = kPass == kHidden ? (V - sum0 < p.split_rows ? V - sum0 : p.split_rows) : kPass == kWeight ? M : D;
+  if (sums < 0) sums = 0;  // a share past the piece's last row: zeros
+  const uint16_t *A, *B;
+  int a_stride, b_stride, a_bytes, b_bytes;
+  if (kPass == kStats || kPass == kGrad) {
+    const int ra = V - r0 < kRows ? V - r0 : kRows, rb = M - c0 < kCols ? M - c0 : kCols;
+    A = p.W + (size_t)r0 * D;
+    B = p.H + (size_t)c0 * D;
+    a_stride = b_stride = D;
+    a_bytes = ra * D * 2;
+    b_bytes = rb * D * 2;
+  } else if (kPass == kHidden) {
+    const int rb = M - c0 < kCols ? M - c0 : kCols;
+    A = p.W + (size_t)sum0 * D + r0;
+    a_stride = D;
+    a_bytes = (sums * D - r0) * 2;
+    B = p.G + (size_t)c0 * p.g_stride + sum0;
+    b_stride = p.g_stride;
+    b_bytes = (rb * p.g_stride - sum0) * 2;
+    if (sums == 0) a_bytes = b_bytes = 0;
+  } else {
+    A = p.H + r0;
+    a_stride = D;
+    a_bytes = (M * D - r0) * 2;
+    B = p.G + c0;
+    b_stride = p.g_stride;
+    b_bytes = (M * p.g_stride - c0) * 2;
+  }
+  const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc((void*)A, (short)0, a_bytes, kBufferWord3);
+  const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void*)B, (short)0, b_bytes, kBufferWord3);
+
+  // fetch offsets and read positions. Rows of 64 (128 bytes): 16-byte chunk c of
+  // row r lands at chunk c ^ (r & 7). Transposed tiles, rows of 256 (512 bytes).
+  uint32_t a_off[4], b_off[T::kFetchB], a_pos[2], b_pos[2], rows_off[4];
+  const uint32_t nat0 = (uint32_t)(j * 128 + ((g ^ (j & 7)) * 16)), nat1 = (uint32_t)(j * 128 + (((4 + g) ^ (j & 7)) * 16));
+  const uint32_t tr0 = (uint32_t)((8 * g + (j >> 2)) * 512 + (j & 3) * 8), tr1 = (uint32_t)(((j >> 2) | ((g & 1) << 2)) * 32);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rows_off[i] = (uint32_t)(8 * wave + 2 * i + (lane >> 5));  // rows of a transposed fetch
+  auto natural = [&](int row, int stride) { return (uint32_t)(row * stride * 2 + ((lane & 7) ^ (lane >> 3)) * 16); };
+  auto turned = [&](int i, int stride, int cols) __attribute__((always_inline)) {
+    const int row = (int)rows_off[i], c = (((lane & 31) >> 1) ^ pair_swizzle(row)) * 2 + (lane & 1);
+    return 8 * c < cols ? (uint32_t)(row * stride * 2 + c * 16) : kBufferOutOfRange;
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    a_off[i] = T::kTrA ? turned(i, a_stride, D - r0) : natural(32 * wave + 8 * i + (lane >> 3), a_stride);
+#pragma unroll
+  for (int i = 0; i < T::kFetchB; ++i)
+    b_off[i] = T::kTrB ? turned(i, b_stride, 256) : natural(kCols / 8 * wave + 8 * i + (lane >> 3), b_stride);
+  a_pos[0] = T::kTrA ? tr0 : nat0;
+  a_pos[1] = T::kTrA ? tr1 : nat1;
+  b_pos[0] = T::kTrB ? tr0 : nat0;
+  b_pos[1] = T::kTrB ? tr1 : nat1;
+
+  f32x4 acc[T::kRT][T::kCT];
+#pragma unroll
+  for (int a = 0; a < T::kRT; ++a) {
+#pragma unroll
+    for (int b = 0; b < T::kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const int nk = (sums + kBlock - 1) / kBlock;
+  // W's rows are read at other columns on other XCDs, which spreads them over the memory channels
+  const int first = kPass == kStats || kPass == kGrad ? (int)(blockIdx.x & 7) * nk / 8 : 0;
+  auto at = [&](int kb) __attribute__((always_inline)) {
+    const int k = (kb < nk ? kb : 0) + first;  // (within the operands also where nothing is fetched)
+    return (uint32_t)(k < nk ? k : k - nk);
+  };
+  const uint32_t a_step = T::kTrA ? (uint32_t)(kBlock * a_stride * 2) : kBlock * 2;
+  const uint32_t b_step = T::kTrB ? (uint32_t)(kBlock * b_stride * 2) : kBlock * 2;
+  // A block past the last is fetched as nothing (zeros); in the last block of a
+  // sum over rows, rows past it are too. (A transposed tile's eight rows of a
+  // wave: whole fetches of two rows, so the row is this lane's.)
+  auto none_of = [&](int kb, bool tr, int i) __attribute__((always_inline)) {
+    if (kb >= nk) return kBufferOutOfRange;
+    return tr && (int)at(kb) * kBlock + (int)rows_off[i] >= sums ? kBufferOutOfRange : 0u;
+  };
+  auto fetch_offsets = [&](int kb, uint32_t (&ao)[4], uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ao[i] = a_off[i] | none_of(kb, T::kTrA, i);
+#pragma unroll
+    for (int i = 0; i < T::kFetchB; ++i) bo[i] = b_off[i] | none_of(kb, T::kTrB, i & 3);
+  };
+#pragma unroll
+  for (int u = 0; u < T::kStages - 1; ++u) {
+    uint32_t ao[4], bo[T::kFetchB];
+    fetch_offsets(u, ao, bo);
+    loss_fetch<4>(ar, lds + u * T::kStage + 4096 * wave, ao, at(u) * a_step, 0);
+    loss_fetch<T::kFetchB>(br, lds + u * T::kStage + T::kA + T::kB / 8 * wave, bo, at(u) * b_step, 0);
+  }
+  for (int kb = 0; kb < nk; kb += T::kStages) {
+#pragma unroll
+    for (int u = 0; u < T::kStages; ++u) {
+      if (kb + u < nk) {
+        // the stage has landed for every wave, and every wave has read the one before
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
+        const int n = kb + u + T::kStages - 1;
+        char* next = lds + (u + T::kStages - 1) % T::kStages * T::kStage;
+        const char* cur = lds + u * T::kStage;
+        uint32_t ao[4], bo[T::kFetchB];
+        fetch_offsets(n, ao, bo);
+        loss_block<kPass, kCols>(cur, cur + T::kA, next + 4096 * wave, next + T::kA + T::kB / 8 * wave, ar, br, ao, bo,
+                                 at(n) * a_step, at(n) * b_step, 0, 0, T::kRT * wr, T::kCT * wc, a_pos, b_pos, acc);
+      }
+    }
+  }
+  // nothing is in flight to or from LDS before the epilogue uses it
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+
+  // lane (j, g) holds rows 16 a + 4 g + e and column 16 b + j of its wave's tile
+  const int row0 = 16 * T::kRT * wr + 4 * g, col0 = 16 * T::kCT * wc + j;
+  if constexpr (kPass == kStats) {
+    const float rcap = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    float2* sums_of = (float2*)lds;  // [kWavesR][kCols]
+#pragma unroll
+    for (int b = 0; b < T::kCT; ++b) {
+      float mx = kLowest;
+#pragma unroll
+      for (int a = 0; a < T::kRT; ++a) {
+        if (p.cap > 0.0f) {
+          float t[4];
+          loss_tanh(acc[a][b], rcap, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[a][b][e] = p.cap * t[e];
+        }
+        if (V - r0 < kRows) {  // (uniform) rows past the vocabulary count nothing
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r0 + row0 + 16 * a + e >= V) acc[a][b][e] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx = __builtin_fmaxf(mx, acc[a][b][e]);
+      }
+      const float ml = mx * kLog2e;
+      float sum = 0.0f;
+#pragma unroll
+      for (int a = 0; a < T::kRT; ++a) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, -ml));
+      }
+      // the four lane groups of a column
+#pragma unroll
+      for (int d = 16; d < 64; d <<= 1) {
+        const float om = __shfl_xor(mx, d), os = __shfl_xor(sum, d);
+        const float nm = __builtin_fmaxf(mx, om);
+        sum = sum * __builtin_amdgcn_exp2f((mx - nm) * kLog2e) + os * __builtin_amdgcn_exp2f((om - nm) * kLog2e);
+        mx = nm;
+      }
+      if (g == 0) sums_of[wr * kCols + col0 + 16 * b] = make_float2(mx, sum);
+    }
+    __syncthreads();
+    if (tid < kCols && c0 + tid < M) {
+      float2 s = sums_of[tid];
+#pragma unroll
+      for (int w = 1; w < T::kWavesR; ++w) {
+        const float2 o = sums_of[w * kCols + tid];
+        const float nm = __builtin_fmaxf(s.x, o.x);
+        s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
+        s.x = nm;
+      }
+      p.stats[(size_t)rt * M + c0 + tid] = s;
+    }
+  } else if constexpr (kPass == kGrad) {
+    const float rcap = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    uint16_t* stage = (uint16_t*)lds;
+#pragma unroll
+    for (int b = 0; b < T::kCT; ++b) {
+      const int col = col0 + 16 * b, m = c0 + col;
+      const int target = m < M ? p.targets[m] : -1;
+      const bool scored = target >= 0 && target < p.vocab;
+      const float ll = m < M ? p.lse[m] * kLog2e : 0.0f;
+      const float d = m < M ? p.dloss[m] : 0.0f;
+      const int hit = target - p.v_base - r0 - row0;  // the target's place among this lane's rows
+      const bool any_hit = __any(target >= 0 && hit >= 0 && hit < 16 * T::kRT);
+#pragma unroll
+      for (int a = 0; a < T::kRT; ++a) {
+        float v[4], t[4];
+        if (p.cap > 0.0f) {
+          loss_tanh(acc[a][b], rcap, t);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = p.cap * t[e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = acc[a][b][e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], kLog2e, -ll));
+        if (any_hit) {  // (uniform)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (hit == 16 * a + e) v[e] -= 1.0f;
+        }
+        if (p.cap > 0.0f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= d * __builtin_fmaf(-t[e], t[e], 1.0f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= d;
+        }
+        if (V - r0 < kRows) {  // (uniform) zeros past the vocabulary
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (r0 + row0 + 16 * a + e >= V) v[e] = 0.0f;
+        }
+        // a row that is not scored has no gradient, whatever its hidden state holds
+        const MxU32x2 w = {scored ? pack_bf16(v[0], v[1]) : 0u, scored ? pack_bf16(v[2], v[3]) : 0u};
+        *(MxU32x2*)&stage[col * T::kOutStride + row0 + 16 * a] = w;
+      }
+    }
+    __syncthreads();
+    // rows of 512 bytes of g
+#pragma unroll 4
+    for (int q = tid; q < kCols * 32; q += kLossThreads) {
+      const int m = q >> 5, c = (q & 31) * 8;
+      if (c0 + m < M)
+        *(MxU32x4*)&p.G[(size_t)(c0 + m) * p.g_stride + r0 + c] = *(const MxU32x4*)&stage[m * T::kOutStride + c];
+    }
+  } else if constexpr (kPass == kHidden) {
+    float* part = p.part + (size_t)split * M * D;
+#pragma unroll
+    for (int b = 0; b < T::kCT; ++b) {
+      const int m = c0 + col0 + 16 * b;
+#pragma unroll
+      for (int a = 0; a < T::kRT; ++a) {
+        const int k = r0 + row0 + 16 * a;
+        if (m < M && k < D) {
+          f32x4* o = (f32x4*)&part[(size_t)m * D + k];
+          f32x4 v = acc[a][b];
+          if (p.accumulate) v += *o;
+          *o = v;
+        }
+      }
+    }
+  } else {
+    uint16_t* stage = (uint16_t*)lds;
+#pragma unroll
+    for (int b = 0; b < T::kCT; ++b) {
+#pragma unroll
+      for (int a = 0; a < T::kRT; ++a) {
+        const f32x4 v = acc[a][b];
+        *(MxU32x2*)&stage[(col0 + 16 * b) * T::kOutStride + row0 + 16 * a] =
+            MxU32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+      }
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int q = tid; q < kCols * 32; q += kLossThreads) {
+      const int v = q >> 5, c = (q & 31) * 8;
+      if (c0 + v < V && r0 + c < D)
+        *(MxU32x4*)&p.dW[(size_t)(c0 + v) * D + r0 + c] = *(const MxU32x4*)&stage[v * T::kOutStride + c];
+    }
+  }
+}
+
+// lse and loss of 8 rows a workgroup: the tiles' (max, sum) joined in one
+// order, and the target's logit as one dot product.
+constexpr int kJoinRows = 8;
+__global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict__ stats, int n_tiles,
+                                                        const uint16_t* __restrict__ H, const uint16_t* __restrict__ W,
+                                                        const int32_t* __restrict__ targets, int M, int D, int V,
+                                                        float cap, float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 slices[32][kJoinRows];
+  __shared__ float lse_of[kJoinRows];
+  const int tid = threadIdx.x, i = tid & (kJoinRows - 1), slice = tid / kJoinRows;
+  const int m0 = (int)blockIdx.x * kJoinRows;
+  float2 s = make_float2(kLowest, 0.0f);
+  if (m0 + i < M) {
+#pragma unroll 4
+    for (int t = slice; t < n_tiles; t += 32) {
+      const float2 o = stats[(size_t)t * M + m0 + i];
+      const float nm = __builtin_fmaxf(s.x, o.x);
+      s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
+      s.x = nm;
+    }
+  }
+  slices[slice][i] = s;
+  __syncthreads();
+  if (slice == 0 && m0 + i < M) {
+    for (int t = 1; t < 32; ++t) {
+      const float2 o = slices[t][i];
+      const float nm = __builtin_fmaxf(s.x, o.x);
+      s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
+      s.x = nm;
+    }
+    const float l = s.x + logf(s.y);
+    lse_of[i] = l;
+    lse[m0 + i] = l;
+  }
+  __syncthreads();
+  const int lane = tid & 63, wave = tid >> 6;
+  for (int r = wave; r < kJoinRows && m0 + r < M; r += 4) {
+    const int64_t t = targets[m0 + r];
+    if (t < 0 || t >= V) {
+      if (lane == 0) loss[m0 + r] = 0.0f;
+      continue;
+    }
+    float z = 0.0f;
+    for (int c = lane * 8; c < D; c += 512) {
+      float x[8], y[8];
+      load_8<true>(H, (int64_t)(m0 + r) * D + c, 8, x);
+      load_8<true>(W, t * D + c, 8, y);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z = __builtin_fmaf(x[e], y[e], z);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) z += __shfl_xor(z, d);
+    if (cap > 0.0f) z = cap * tanhf(z / cap);
+    if (lane == 0) loss[m0 + r] = lse_of[r] - z;
+  }
+}
+
+// H with zeros in the rows that are not scored, for dW's product (their g is
+// zero, but zero times what a padded row may hold need not be).
+__global__ __launch_bounds__(256) void loss_rows_kernel(const uint16_t* __restrict__ H,
+                                                        const int32_t* __restrict__ targets, int V, int D, int64_t n,
+                                                        uint16_t* __restrict__ out) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= n) return;
+  const int t = targets[e / D];
+  const MxU32x4 z = {0, 0, 0, 0};
+  *(MxU32x4*)&out[e] = t >= 0 && t < V ? *(const MxU32x4*)&H[e] : z;
+}
+
+// dH = the shares, added in order and rounded once.
+__global__ __launch_bounds__(256) void loss_hidden_kernel(const float* __restrict__ part, int splits, int64_t n,
+                                                          uint16_t* __restrict__ dH) {
+  const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  if (e >= n) return;
+  float v[8];
+  load_8<false>(part, e, 8, v);
+  for (int s = 1; s < splits; ++s) {
+    float o[8];
+    load_8<false>(part, s * n + e, 8, o);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += o[i];
+  }
+  store_8<true>(dH, e, 8, v);
+}
+
+template <Pass kPass>
+void loss_launch(const LossArgs& p, int cols, hipStream_t s) {
+  const int total = p.row_tiles * p.col_tiles * p.splits;
+  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(kLossThreads);
+  if constexpr (kPass == kWeight) {
+    loss_kernel<kPass, 256><<<grid, block, 0, s>>>(p);
+  } else if (cols == 64) {
+    loss_kernel<kPass, 64><<<grid, block, 0, s>>>(p);
+  } else if (cols == 128) {
+    loss_kernel<kPass, 128><<<grid, block, 0, s>>>(p);
+  } else {
+    loss_kernel<kPass, 256><<<grid, block, 0, s>>>(p);
+  }
+}
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+}  // namespace
+
+LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count) {
+  LossPlan q{};
+  q.cols = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  q.v_tiles = (vocab + kRows - 1) / kRows;
+  // a piece: at most 256 MB of g, and its offsets (and W's) within 31 bits
+  int64_t piece = ((int64_t)256 << 20) / ((int64_t)rows * 2);
+  piece = std::min<int64_t>(piece, ((int64_t)1 << 30) / width - 256);
+  piece = std::max<int64_t>(256, piece / 256 * 256);
+  q.piece = (int32_t)std::min<int64_t>(piece, (int64_t)q.v_tiles * 256);
+  const int tiles = (width + kRows - 1) / kRows * ((rows + q.cols - 1) / q.cols);
+  const int cus = cu_count > 0 ? cu_count : 256;
+  q.splits = std::max(1, std::min(cus / tiles, q.piece / 256));
+  q.stats_bytes = up256((size_t)q.v_tiles * rows * sizeof(float2));
+  q.g_bytes = up256((size_t)rows * q.piece * 2);
+  q.h_bytes = up256((size_t)rows * width * 2);
+  q.part_bytes = up256((size_t)q.splits * rows * width * 4);
+  return q;
+}
+
+void launch_lmhead_loss(const uint16_t* hidden, const uint16_t* weight, const int32_t* targets, int32_t rows,
+                        int32_t width, int32_t vocab, float softcap, const LossPlan& plan, uint8_t* work, float* loss,
+                        float* lse, hipStream_t s) {
+  LossArgs p{};
+  p.W = weight;
+  p.H = hidden;
+  p.stats = (float2*)work;
+  p.cap = softcap;
+  p.M = rows;
+  p.D = width;
+  p.V = vocab;
+  p.row_tiles = plan.v_tiles;
+  p.col_tiles = (rows + plan.cols - 1) / plan.cols;
+  p.splits = 1;
+  loss_launch<kStats>(p, plan.cols, s);
+  loss_join_kernel<<<dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(256), 0, s>>>(
+      p.stats, plan.v_tiles, hidden, weight, targets, rows, width, vocab, softcap, loss, lse);
+}
+
+void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, const int32_t* targets, const float* lse,
+                             const float* dloss, int32_t rows, int32_t width, int32_t vocab, float softcap,
+                             const LossPlan& plan, uint8_t* work, uint16_t* dhidden, uint16_t* dweight, hipStream_t s) {
+  const int64_t n = (int64_t)rows * width;
+  const dim3 per8((unsigned)((n / 8 + 255) / 256)), block(256);
+  uint16_t* scored = (uint16_t*)(work + plan.g_bytes);
+  float* part = (float*)(work + plan.g_bytes + plan.h_bytes);
+  if (dweight) loss_rows_kernel<<<per8, block, 0, s>>>(hidden, targets, vocab, width, n, scored);
+  const int k_tiles = (width + kRows - 1) / kRows;
+  int splits = 1;
+  for (int32_t v = 0; v < vocab; v += plan.piece) {
+    LossArgs p{};
+    p.W = weight + (size_t)v * width;
+    p.H = hidden;
+    p.G = (uint16_t*)work;
+    p.targets = targets;
+    p.lse = lse;
+    p.dloss = dloss;
+    p.part = part;
+    p.cap = softcap;
+    p.M = rows;
+    p.D = width;
+    p.V = std::min(plan.piece, vocab - v);
+    p.v_base = v;
+    p.vocab = vocab;
+    p.g_stride = (p.V + 255) / 256 * 256;
+    p.row_tiles = p.g_stride / 256;
+    p.col_tiles = (rows + plan.cols - 1) / plan.cols;
+    p.splits = 1;
+    loss_launch<kGrad>(p, plan.cols, s);
+    if (dhidden) {
+      // every piece fills the same shares: the last, shorter one in shorter runs
+      p.row_tiles = k_tiles;
+      if (v == 0) splits = std::min(plan.splits, p.g_stride / 256);
+      p.splits = splits;
+      p.split_rows = ((p.V + splits - 1) / splits + kBlock - 1) / kBlock * kBlock;
+      p.accumulate = v > 0;
+      loss_launch<kHidden>(p, plan.cols, s);
+    }
+    if (dweight) {
+      p.H = scored;
+      p.dW = dweight + (size_t)v * width;
+      p.row_tiles = k_tiles;
+      p.col_tiles = p.g_stride / 256;
+      p.splits = 1;
+      loss_launch<kWeight>(p, 256, s);
+    }
+  }
+  if (dhidden) loss_hidden_kernel<<<per8, block, 0, s>>>(part, splits, n, dhidden);
+}
+
+}  // namespace gs

@@ -1,0 +1,157 @@
+// Microscaled blocks: 32 values share one power of two (E8M0, bias 127, 255
+// for a block that holds a NaN or an infinity) and are held in e2m1 (4 bits)
+// or e4m3 (8 bits). The shared exponent is floor(log2 of the block's largest
+// magnitude) less the element format's largest exponent (2 or 8), at least
+// -127, so the largest magnitude lands in the format's top binade; what lies
+// past its largest value there (6 or 448) becomes that value, everything else
+// is rounded to nearest, ties to the even mantissa. The 8-bit and the 4-bit
+// values of a block hold relative errors of 2^-4 and 2^-2 at most above the
+// format's smallest normal value: that is the choice of the formats.
+#pragma once
+
+#include "gs_internal.h"
+
+namespace gs {
+
+constexpr int kMxBlock = 32;
+
+typedef uint32_t MxU32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t MxU32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any element's alignment (rows of odd strides)
+typedef uint32_t MxU32x4Any __attribute__((ext_vector_type(4), aligned(2)));
+
+// 8 values of a row from element `e` on, `n` of them inside the row (zeros past it).
+template <bool kBf16>
+__device__ __forceinline__ void load_8(const void* p, int64_t e, int n, float (&v)[8]) {
+  if (kBf16) {
+    const uint16_t* q = (const uint16_t*)p + e;
+    if (n >= 8) {
+      const MxU32x4Any u = *(const MxU32x4Any*)q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(u[i] << 16);
+        v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? __uint_as_float((uint32_t)q[i] << 16) : 0.0f;
+    }
+  } else {
+    const float* q = (const float*)p + e;
+    if (n >= 8) {
+      typedef float F32x4Any __attribute__((ext_vector_type(4), aligned(4)));
+      const F32x4Any a = *(const F32x4Any*)q, b = *(const F32x4Any*)(q + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = i < n ? q[i] : 0.0f;
+    }
+  }
+}
+
+// Two floats as bf16, each rounded to nearest even (half a step, 2^-9 of the value's binade top).
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
+  const Bf16x2 p = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(uint32_t, p);
+}
+
+template <bool kBf16>
+__device__ __forceinline__ float rounded_to(float x) {
+  return kBf16 ? (float)(__bf16)x : x;
+}
+
+template <bool kBf16>
+__device__ __forceinline__ void store_8(void* p, int64_t e, int n, const float (&v)[8]) {
+  if (kBf16) {
+    uint16_t* q = (uint16_t*)p + e;
+    const MxU32x4Any u = {pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7])};
+    if (n >= 8) {
+      *(MxU32x4Any*)q = u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = (uint16_t)(u[i / 2] >> (16 * (i & 1)));
+    }
+  } else {
+    float* q = (float*)p + e;
+    typedef float F32x4Any __attribute__((ext_vector_type(4), aligned(4)));
+    if (n >= 8) {
+      *(F32x4Any*)q = F32x4Any{v[0], v[1], v[2], v[3]};
+      *(F32x4Any*)(q + 4) = F32x4Any{v[4], v[5], v[6], v[7]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < n) q[i] = v[i];
+    }
+  }
+}
+
+// The scale code of a block from the bits of its largest magnitude: a NaN's
+// bits are above an infinity's, so an integer maximum keeps either.
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t amax_bits, int emax) {
+  const int e = (int)(amax_bits >> 23);
+  return e == 255 ? 255u : (uint32_t)(e > emax ? e - emax : 0);
+}
+
+// 2^(127 - code): the factor that brings a block's values into the element
+// format's range (exact for every code below 255 of a finite block).
+__device__ __forceinline__ float mx_inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
+// 2^(code - 127), a subnormal for code 0, NaN for 255.
+__device__ __forceinline__ float mx_scale(uint32_t code) {
+  return code == 0 ? __uint_as_float(0x00400000u) : code == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(code << 23);
+}
+
+// The largest magnitude's bits over the four lanes that hold a block's 32
+// values (8 each, lanes 4k .. 4k + 3).
+__device__ __forceinline__ uint32_t mx_block_amax(const float (&v)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    m = b > m ? b : m;
+  }
+#pragma unroll
+  for (int d = 1; d < 4; d <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+    m = o > m ? o : m;
+  }
+  return m;
+}
+
+// 8 values at the block's scale as e4m3 codes (a special block: NaN codes).
+__device__ __forceinline__ MxU32x2 mx_codes_e4m3(const float (&v)[8], uint32_t code) {
+  if (code == 255) return MxU32x2{0x7f7f7f7fu, 0x7f7f7f7fu};
+  const float s = mx_inverse_scale(code);
+  int lo = 0, hi = 0;
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_fmed3f(v[i] * s, -448.0f, 448.0f);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], lo, false);
+  lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], hi, false);
+  hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], hi, true);
+  return MxU32x2{(uint32_t)lo, (uint32_t)hi};
+}
+
+// 8 values at the block's scale as e2m1 codes, the first in the low bits (a
+// special block: zeros, its scale says NaN).
+__device__ __forceinline__ uint32_t mx_codes_e2m1(const float (&v)[8], uint32_t code) {
+  if (code == 255) return 0u;
+  const float s = mx_inverse_scale(code);
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_fmed3f(v[i] * s, -6.0f, 6.0f);
+  uint32_t u = 0;
+  u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, q[0], q[1], 1.0f, 0);
+  u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, q[2], q[3], 1.0f, 1);
+  u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, q[4], q[5], 1.0f, 2);
+  u = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(u, q[6], q[7], 1.0f, 3);
+  return u;
+}
+
+}  // namespace gs

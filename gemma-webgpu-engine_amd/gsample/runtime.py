@@ -24,6 +24,8 @@ LIB_PATH = os.path.join(PKG, "lib", "libgsample_checked.so" if os.environ.get("G
 
 GS_F32, GS_BF16 = 0, 1
 GS_QAT_ROW_MAJOR, GS_QAT_BLOCK_MAJOR = 0, 1
+GS_MX_E2M1, GS_MX_E4M3 = 0, 1
+MX_FORMATS = {"e2m1": GS_MX_E2M1, "e4m3": GS_MX_E4M3}
 GS_RNG_SEEDED, GS_RNG_EXPLICIT = 0, 1
 GS_ROW_FORCE_EXACT = 1
 GS_BATCH_FULL_DRAWS = 1  # gs_batch.hints: a row may take a full-vocabulary draw
@@ -116,7 +118,8 @@ EXPORTED_SYMBOLS = (
     "gs_validate_configs", "gs_create", "gs_destroy", "gs_last_error", "gs_synchronize", "gs_stream",
     "gs_sample", "gs_sample_noalloc", "gs_sample_sync", "gs_token_log_prob", "gs_token_log_prob_host", "gs_set_vocab", "gs_set_dfa",
     "gs_build_masks", "gs_dfa_advance", "gs_dfa_accepting", "gs_lmhead", "gs_lmhead_sample", "gs_qat_lmhead", "gs_qat_lmhead_sample", "gs_timing_begin",
-    "gs_timing_end", "gs_check_exp2",
+    "gs_timing_end", "gs_check_exp2", "gs_rms_norm", "gs_rms_norm_grad", "gs_mx_quantize", "gs_mx_dequantize",
+    "gs_mx_lmhead", "gs_mx_lmhead_sample", "gs_lmhead_loss", "gs_lmhead_loss_grad",
 )
 
 # kernel stages reported by gs_timing_end (include/gsample.h GS_STAGE_*)
@@ -169,6 +172,15 @@ def library():
     L.gs_timing_begin.argtypes = [vp, i32]
     L.gs_timing_end.argtypes = [vp, vp, vp]
     L.gs_check_exp2.argtypes = [vp, C.c_float, C.c_float, C.POINTER(C.c_double), C.POINTER(C.c_float)]
+    f32 = C.c_float
+    L.gs_rms_norm.argtypes = [vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, f32, f32, vp, vp, vp, vp, vp]
+    L.gs_rms_norm_grad.argtypes = [vp, vp, vp, vp, vp, i32, i32, i32, i32, i64, i64, i64, f32, f32, vp, vp, vp]
+    L.gs_mx_quantize.argtypes = [vp, vp, i32, i32, i64, i32, i64, vp, vp, vp]
+    L.gs_mx_dequantize.argtypes = [vp, vp, vp, i32, i64, i32, i32, vp, vp]
+    L.gs_mx_lmhead.argtypes = [vp, vp, vp, vp, vp, i32, i32, f32, vp, vp]
+    L.gs_mx_lmhead_sample.argtypes = [vp, vp, vp, vp, vp, i32, f32, vp, C.POINTER(Batch), vp]
+    L.gs_lmhead_loss.argtypes = [vp, vp, vp, vp, i32, i32, f32, vp, vp, vp]
+    L.gs_lmhead_loss_grad.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, f32, vp, vp, vp]
     _lib = L
     return L
 
@@ -552,6 +564,257 @@ class Sampler:
         self._check(self.lib.gs_lmhead_sample(self.ctx, C.c_void_p(hidden.data_ptr()), C.c_void_p(weight.data_ptr()),
                                               width, float(softcap_value), C.c_void_p(logits_scratch.data_ptr()),
                                               C.byref(batch), C.c_void_p(stream or 0)))
+
+
+    # -- the operators on either side of the head ------------------------
+    # Each takes the memory of its results (allocated when left out) and a
+    # stream. With a stream it enqueues there and returns; inputs must be ready
+    # on that stream. Without one it waits for torch's current stream, runs on
+    # the context's and waits for the results.
+    def _tensor(self, t, name: str, dtype, shape=None):
+        """The pointer of a checked contiguous tensor (None: NULL)."""
+        if t is None:
+            return None
+        dtypes = dtype if isinstance(dtype, tuple) else (dtype,)
+        if t.dtype not in dtypes:
+            raise GSampleError(1, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
+        if t.device != self.device:
+            raise GSampleError(1, f"{name} must live on the sampler's device")
+        if shape is not None and tuple(t.shape) != tuple(shape):
+            raise GSampleError(1, f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise GSampleError(1, f"{name} must be contiguous")
+        return t.data_ptr()
+
+    def _rows(self, t, name: str, dtype, shape=None):
+        """(pointer, row stride) of a checked tensor of rows (None: NULL)."""
+        if t is None:
+            return None, 0
+        dtypes = dtype if isinstance(dtype, tuple) else (dtype,)
+        if t.dtype not in dtypes:
+            raise GSampleError(1, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
+        if t.device != self.device:
+            raise GSampleError(1, f"{name} must live on the sampler's device")
+        if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+            raise GSampleError(1, f"{name} must have shape {tuple(shape) if shape else '(rows, width)'}, "
+                                  f"not {tuple(t.shape)}")
+        rows, width = t.shape
+        if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
+            raise GSampleError(1, f"{name}'s rows must be contiguous and not overlap")
+        return t.data_ptr(), t.stride(0)
+
+    def _empty(self, shape, dtype, stream):
+        """Memory for a result of a call on `stream`: the caching allocator must
+        not hand it out again before that stream has used it."""
+        t = self.torch.empty(shape, dtype=dtype, device=self.device)
+        if stream is not None and self.torch.cuda.current_stream(self.device).cuda_stream != stream:
+            t.record_stream(self.torch.cuda.ExternalStream(stream, device=self.device))
+        return t
+
+    def _begin(self, stream):
+        if stream is None:
+            self.torch.cuda.current_stream(self.device).synchronize()
+        return stream or None
+
+    def _end(self, stream):
+        if stream is None:
+            self.synchronize()
+
+    def rms_norm(self, x, weight, residual=None, eps: float = 1e-6, weight_offset: float = 0.0, out=None, summed=None,
+                 codes=None, scales=None, stream: Optional[int] = None):
+        """gs_rms_norm: y = h (weight_offset + weight) / sqrt(mean(h^2) + eps) with
+        h = x + residual rounded to x's type. x, residual: f32 or bf16 [rows][width].
+        Returns y, in `out` (x's type) or, where `codes` and `scales` (uint8
+        [rows][width] and [rows][width / 32]) are given, written there in e4m3 blocks
+        (then `out` is written too only if it is given, and the return value is
+        (codes, scales)). h goes to `summed` where that is given."""
+        torch = self.torch
+        kinds = (torch.float32, torch.bfloat16)
+        px, x_stride = self._rows(x, "x", kinds)
+        rows, width = (int(n) for n in x.shape)
+        pr, r_stride = self._rows(residual, "residual", x.dtype, (rows, width))
+        pw = self._tensor(weight, "weight", kinds, (width,))
+        if (codes is None) != (scales is None):
+            raise GSampleError(1, "codes and scales go together")
+        if out is None and codes is None:
+            out = self._empty((rows, width), x.dtype, stream)
+        po = self._tensor(out, "out", x.dtype, (rows, width))
+        ps = self._tensor(summed, "summed", x.dtype, (rows, width))
+        pc = self._tensor(codes, "codes", torch.uint8, (rows, width))
+        psc = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
+        s = self._begin(stream)
+        self._check(self.lib.gs_rms_norm(
+            self.ctx, px, pr, pw, GS_BF16 if x.dtype == torch.bfloat16 else GS_F32,
+            GS_BF16 if weight.dtype == torch.bfloat16 else GS_F32, rows, width, x_stride, r_stride, float(eps),
+            float(weight_offset), ps, po, pc, psc, s))
+        self._end(stream)
+        return out if codes is None else (codes, scales)
+
+    def rms_norm_grad(self, dy, summed, weight, dsummed=None, eps: float = 1e-6, weight_offset: float = 0.0, dx=None,
+                      dweight=None, stream: Optional[int] = None):
+        """gs_rms_norm_grad: (dx, dweight) from dy, the norm's h (its `summed`, or x without
+        a residual) and, if the residual stream goes on, its gradient dsummed. dx (of dy's
+        type) is the gradient of x and of the residual; dweight is f32 [width]."""
+        torch = self.torch
+        kinds = (torch.float32, torch.bfloat16)
+        ph, h_stride = self._rows(summed, "summed", kinds)
+        rows, width = (int(n) for n in summed.shape)
+        pd, d_stride = self._rows(dy, "dy", summed.dtype, (rows, width))
+        pds, ds_stride = self._rows(dsummed, "dsummed", summed.dtype, (rows, width))
+        pw = self._tensor(weight, "weight", kinds, (width,))
+        if dx is None:
+            dx = self._empty((rows, width), summed.dtype, stream)
+        if dweight is None:
+            dweight = self._empty((width,), torch.float32, stream)
+        px = self._tensor(dx, "dx", summed.dtype, (rows, width))
+        pdw = self._tensor(dweight, "dweight", torch.float32, (width,))
+        s = self._begin(stream)
+        self._check(self.lib.gs_rms_norm_grad(
+            self.ctx, pd, ph, pw, pds, GS_BF16 if summed.dtype == torch.bfloat16 else GS_F32,
+            GS_BF16 if weight.dtype == torch.bfloat16 else GS_F32, rows, width, d_stride, h_stride, ds_stride,
+            float(eps), float(weight_offset), px, pdw, s))
+        self._end(stream)
+        return dx, dweight
+
+    def _mx_format(self, fmt: str) -> int:
+        if fmt not in MX_FORMATS:
+            raise GSampleError(1, f"format must be one of {', '.join(sorted(MX_FORMATS))}")
+        return MX_FORMATS[fmt]
+
+    def mx_quantize(self, x, fmt: str, codes=None, scales=None, stream: Optional[int] = None):
+        """gs_mx_quantize: (codes, scales) of x (f32 or bf16 [rows][width]) in blocks of 32;
+        fmt "e2m1" (codes uint8 [rows][width / 2]) or "e4m3" ([rows][width])."""
+        torch = self.torch
+        f = self._mx_format(fmt)
+        px, x_stride = self._rows(x, "x", (torch.float32, torch.bfloat16))
+        rows, width = (int(n) for n in x.shape)
+        shape = (rows, width // 2 if f == GS_MX_E2M1 else width)
+        if codes is None:
+            codes = self._empty(shape, torch.uint8, stream)
+        if scales is None:
+            scales = self._empty((rows, width // 32), torch.uint8, stream)
+        pc = self._tensor(codes, "codes", torch.uint8, shape)
+        ps = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
+        s = self._begin(stream)
+        self._check(self.lib.gs_mx_quantize(self.ctx, px, GS_BF16 if x.dtype == torch.bfloat16 else GS_F32, f, rows,
+                                            width, x_stride, pc, ps, s))
+        self._end(stream)
+        return codes, scales
+
+    def mx_dequantize(self, codes, scales, fmt: str, out=None, dtype=None, stream: Optional[int] = None):
+        """gs_mx_dequantize: the values of codes and scales, in `out` or in new memory of
+        `dtype` (torch.bfloat16, the default, or torch.float32)."""
+        torch = self.torch
+        f = self._mx_format(fmt)
+        pc = self._tensor(codes, "codes", torch.uint8)
+        if codes.dim() != 2:
+            raise GSampleError(1, "codes must have two dimensions")
+        rows, width = int(codes.shape[0]), int(codes.shape[1]) * (2 if f == GS_MX_E2M1 else 1)
+        ps = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
+        if out is None:
+            out = self._empty((rows, width), torch.bfloat16 if dtype is None else dtype, stream)
+        po = self._tensor(out, "out", (torch.float32, torch.bfloat16), (rows, width))
+        s = self._begin(stream)
+        self._check(self.lib.gs_mx_dequantize(self.ctx, pc, ps, f, rows, width,
+                                              GS_BF16 if out.dtype == torch.bfloat16 else GS_F32, po, s))
+        self._end(stream)
+        return out
+
+    def _mx_head(self, hidden, hidden_scales, weight, weight_scales):
+        """The checked pointers and sizes of the 4-bit head's operands."""
+        u8 = self.torch.uint8
+        ph = self._tensor(hidden, "hidden", u8)
+        if hidden.dim() != 2:
+            raise GSampleError(1, "hidden must have shape (rows, width)")
+        m, width = (int(n) for n in hidden.shape)
+        phs = self._tensor(hidden_scales, "hidden_scales", u8, (m, width // 32))
+        pw = self._tensor(weight, "weight", u8, (self.vocab, width // 2))
+        pws = self._tensor(weight_scales, "weight_scales", u8, (self.vocab, width // 32))
+        return ph, phs, pw, pws, m, width
+
+    def mx_lmhead(self, hidden, hidden_scales, weight, weight_scales, softcap_value: float = 0.0, out=None,
+                  stream: Optional[int] = None):
+        """gs_mx_lmhead: f32 logits [rows][V] of e4m3 hidden states and e2m1 weights, codes and
+        scales as mx_quantize (or rms_norm) writes them."""
+        ph, phs, pw, pws, m, width = self._mx_head(hidden, hidden_scales, weight, weight_scales)
+        if out is None:
+            out = self._empty((m, self.vocab), self.torch.float32, stream)
+        po = self._tensor(out, "out", self.torch.float32, (m, self.vocab))
+        s = self._begin(stream)
+        self._check(self.lib.gs_mx_lmhead(self.ctx, ph, phs, pw, pws, m, width, float(softcap_value), po, s))
+        self._end(stream)
+        return out
+
+    def mx_lmhead_sample(self, hidden, hidden_scales, weight, weight_scales, softcap_value: float, logits_scratch,
+                         configs: np.ndarray, histories=None, forced=None, mask_table=None) -> "SampleOutput":
+        """gs_mx_lmhead_sample: the 4-bit head into `logits_scratch` ([rows][V] f32), then the
+        sampler on it, one call; returns the rows' results."""
+        b, keep = self.prepare(logits_scratch, configs, histories, forced, mask_table)
+        self.mx_lmhead_sample_launch(hidden, hidden_scales, weight, weight_scales, softcap_value, logits_scratch, b)
+        self.synchronize()
+        res = keep[-1].cpu().numpy().view(np.uint8).reshape(-1)[: b.rows * 16].view(RESULT_DTYPE)
+        del keep
+        return SampleOutput(res["token"].copy(), res["probability"].copy(), res["flags"].copy())
+
+    def mx_lmhead_sample_launch(self, hidden, hidden_scales, weight, weight_scales, softcap_value: float,
+                                logits_scratch, batch: Batch, stream: Optional[int] = None):
+        """gs_mx_lmhead_sample: the 4-bit head into `logits_scratch`, then the sampler on it."""
+        ph, phs, pw, pws, m, width = self._mx_head(hidden, hidden_scales, weight, weight_scales)
+        if m != batch.rows:
+            raise GSampleError(1, "one hidden row per row of the batch")
+        po = self._tensor(logits_scratch, "logits_scratch", self.torch.float32, (m, self.vocab))
+        s = self._begin(stream)
+        self._check(self.lib.gs_mx_lmhead_sample(self.ctx, ph, phs, pw, pws, width, float(softcap_value), po,
+                                                 C.byref(batch), s))
+
+    def _loss_operands(self, hidden, weight, targets):
+        torch = self.torch
+        ph = self._tensor(hidden, "hidden", torch.bfloat16)
+        if hidden.dim() != 2:
+            raise GSampleError(1, "hidden must have shape (rows, width)")
+        rows, width = (int(n) for n in hidden.shape)
+        pw = self._tensor(weight, "weight", torch.bfloat16, (self.vocab, width))
+        pt = self._tensor(targets, "targets", torch.int32, (rows,))
+        return ph, pw, pt, rows, width
+
+    def lmhead_loss(self, hidden, weight, targets, softcap_value: float = 0.0, loss=None, lse=None,
+                    stream: Optional[int] = None):
+        """gs_lmhead_loss: (loss, lse), f32 [rows]: each row's cross entropy against its target
+        (int32; outside [0, V): not scored, loss 0) under the bf16 head with the softcap, and
+        the logarithm of its sum of exponentials. No logits are written."""
+        f32 = self.torch.float32
+        ph, pw, pt, rows, width = self._loss_operands(hidden, weight, targets)
+        if loss is None:
+            loss = self._empty((rows,), f32, stream)
+        if lse is None:
+            lse = self._empty((rows,), f32, stream)
+        pl, pe = self._tensor(loss, "loss", f32, (rows,)), self._tensor(lse, "lse", f32, (rows,))
+        s = self._begin(stream)
+        self._check(self.lib.gs_lmhead_loss(self.ctx, ph, pw, pt, rows, width, float(softcap_value), pl, pe, s))
+        self._end(stream)
+        return loss, lse
+
+    def lmhead_loss_grad(self, hidden, weight, targets, lse, dloss, softcap_value: float = 0.0, dhidden=None,
+                         dweight=None, hidden_grad: bool = True, weight_grad: bool = True,
+                         stream: Optional[int] = None):
+        """gs_lmhead_loss_grad: (dhidden, dweight), bf16, for dloss (f32 [rows]) and the lse that
+        lmhead_loss gave for the same operands. hidden_grad / weight_grad False: that one is
+        not computed (None)."""
+        torch = self.torch
+        ph, pw, pt, rows, width = self._loss_operands(hidden, weight, targets)
+        pe = self._tensor(lse, "lse", torch.float32, (rows,))
+        pl = self._tensor(dloss, "dloss", torch.float32, (rows,))
+        if dhidden is None and hidden_grad:
+            dhidden = self._empty((rows, width), torch.bfloat16, stream)
+        if dweight is None and weight_grad:
+            dweight = self._empty((self.vocab, width), torch.bfloat16, stream)
+        pdh = self._tensor(dhidden if hidden_grad else None, "dhidden", torch.bfloat16, (rows, width))
+        pdw = self._tensor(dweight if weight_grad else None, "dweight", torch.bfloat16, (self.vocab, width))
+        s = self._begin(stream)
+        self._check(self.lib.gs_lmhead_loss_grad(self.ctx, ph, pw, pt, pe, pl, rows, width, float(softcap_value), pdh,
+                                                 pdw, s))
+        self._end(stream)
+        return dhidden if hidden_grad else None, dweight if weight_grad else None
 
 
 _default_sampler: Optional[Sampler] = None

@@ -320,6 +320,97 @@ int gs_qat_lmhead_sample(gs_context* ctx, const float* x, int32_t width, const u
                          int32_t layout, const float* row_scales, float input_scale, float output_scale,
                          float* logits_scratch, const gs_batch* batch, void* stream);
 
+/* The operators on either side of the head. All pointers are device memory of
+ * the context's device; every call enqueues on `stream` (NULL: the context's)
+ * and, but for the two that say so, needs no memory of the context. Rows are
+ * not limited by max_rows, and no rows is no work. Outputs are contiguous; an
+ * output may be the same memory as a contiguous input of its shape and type,
+ * and must not overlap an input in any other way. */
+
+/* Root-mean-square norm with the residual's addition (the block's last sum and
+ * the final norm that feeds the head):
+ *   h = x + residual, rounded to dtype (h = x without a residual)
+ *   y = h * (weight_offset + weight) / sqrt(mean(h^2) + eps)
+ * x, residual: [rows][width] of dtype, rows x_stride / residual_stride elements
+ * apart; weight [width] of weight_dtype. Written where given: summed (h), out
+ * (y in dtype), and codes + scales: y in e4m3 blocks as gs_mx_quantize lays
+ * them out, rounded once from binary32 (width a multiple of 32, codes 16-byte
+ * aligned). width at most 16384. */
+int gs_rms_norm(gs_context* ctx, const void* x, const void* residual, const void* weight, int32_t dtype,
+                int32_t weight_dtype, int32_t rows, int32_t width, int64_t x_stride, int64_t residual_stride,
+                float eps, float weight_offset, void* summed, void* out, uint8_t* codes, uint8_t* scales, void* stream);
+
+/* Its gradients from dy (the gradient of y) and h (gs_rms_norm's `summed`, or x
+ * without a residual):
+ *   dx = r (g - h r^2 mean(g h)) + dsummed,  g = dy (weight_offset + weight),
+ *   dweight = sum over rows of dy h r (f32 [width]),  r = 1 / sqrt(mean(h^2) + eps)
+ * dx is the gradient of x and of the residual; dsummed (NULL: none) is the
+ * gradient that reaches h by the residual stream. dx or dweight may be NULL.
+ * dweight's partial sums take the context's work memory (see
+ * gs_lmhead_loss_grad). No rows: dweight is zero. */
+int gs_rms_norm_grad(gs_context* ctx, const void* dy, const void* h, const void* weight, const void* dsummed,
+                     int32_t dtype, int32_t weight_dtype, int32_t rows, int32_t width, int64_t dy_stride,
+                     int64_t h_stride, int64_t dsummed_stride, float eps, float weight_offset, void* dx,
+                     float* dweight, void* stream);
+
+/* Microscaled blocks (the OCP MX formats): 32 neighbouring values of a row share
+ * a power of two, 2^(scale - 127) with scale = floor(log2(largest magnitude)) -
+ * emax + 127, at least 0, and are rounded to nearest even in the element format,
+ * the largest value kept: e2m1 (emax 2, values up to 6; two codes a byte, the
+ * first in the low half) or e4m3 (emax 8, up to 448; a byte each). A block with a
+ * NaN or an infinity gets scale 255 and reads back as NaN.
+ * x: [rows][width] of dtype, rows row_stride elements apart; codes
+ * [rows][width / 2] or [rows][width] and scales [rows][width / 32], contiguous,
+ * codes 16-byte aligned. width a multiple of 32. */
+#define GS_MX_E2M1 0
+#define GS_MX_E4M3 1
+int gs_mx_quantize(gs_context* ctx, const void* x, int32_t dtype, int32_t format, int64_t rows, int32_t width,
+                   int64_t row_stride, uint8_t* codes, uint8_t* scales, void* stream);
+/* The values that codes and scales stand for, in dtype (exact in both, but for
+ * magnitudes below its normal numbers). out [rows][width], 16-byte aligned. */
+int gs_mx_dequantize(gs_context* ctx, const uint8_t* codes, const uint8_t* scales, int32_t format, int64_t rows,
+                     int32_t width, int32_t dtype, void* out, void* stream);
+
+/* The lm_head over microscaled operands: logits[m][v] = cap(hidden[m] . weight[v])
+ * with hidden in e4m3 ([m_rows][width], scales [m_rows][width / 32]) and weight in
+ * e2m1 ([V][width / 2], scales [V][width / 32]), both as gs_mx_quantize lays them
+ * out, sums in binary32, the cap as gs_lmhead's. width a multiple of 64, at most
+ * 16384; codes 16-byte, scales 2-byte aligned. logits f32 [m_rows][V]. */
+int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
+                 const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t m_rows, int32_t width,
+                 float softcap, float* logits, void* stream);
+/* gs_mx_lmhead followed by gs_sample on its output, as gs_qat_lmhead_sample. */
+int gs_mx_lmhead_sample(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
+                        const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t width, float softcap,
+                        float* logits_scratch, const gs_batch* batch, void* stream);
+
+/* Softmax cross entropy of the head's logits z = cap(hidden . weight) (gs_lmhead's,
+ * never written to memory): lse[m] = log(sum_v exp(z[m][v])) and
+ * loss[m] = lse[m] - z[m][targets[m]], 0 where the target is outside [0, V) (a
+ * row that is not scored). hidden bf16 [rows][width], weight bf16 [V][width],
+ * 16-byte aligned, width a multiple of 64; targets int32 [rows]; loss and lse f32
+ * [rows]. width at most 65536, rows at most 2^20, rows * width below 2^30. Takes the
+ * context's work memory. */
+int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets, int32_t rows,
+                   int32_t width, float softcap, float* loss, float* lse, void* stream);
+/* Its gradients for dloss (f32 [rows], the gradient of loss; not read where a row
+ * is not scored) from the lse that gs_lmhead_loss wrote for the same operands:
+ *   g[m][v] = dloss[m] (exp(z[m][v] - lse[m]) - [v = targets[m]]) (1 - (z[m][v] / cap)^2)
+ *   dhidden = g . weight (bf16 [rows][width]),  dweight = g^T . hidden (bf16 [V][width])
+ * A row that is not scored adds nothing, whatever its hidden state holds. dhidden or
+ * dweight may be NULL; both are 16-byte aligned. g is made again a piece of the
+ * vocabulary at a time and rounded to bf16 for the two products, whose sums are in
+ * binary32. No rows: dweight is zero.
+ * Work memory: gs_lmhead_loss, gs_lmhead_loss_grad and gs_rms_norm_grad share one
+ * allocation of the context, which the largest call so far sized; it is not given
+ * back before gs_destroy. Calls that take it must be ordered on one stream, and
+ * graphs that hold such calls must not run side by side. A call that would have to
+ * enlarge it on a stream under capture returns GS_ERR_UNSUPPORTED: make the call
+ * once before the capture. */
+int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets,
+                        const float* lse, const float* dloss, int32_t rows, int32_t width, float softcap,
+                        void* dhidden, void* dweight, void* stream);
+
 /* Self-check of the bound the chunk scan's normaliser rests on; no
  * counterpart in the reference. Largest relative error of the hardware
  * binary32 exp2 (v_exp_f32, which the scan evaluates every term with) over
