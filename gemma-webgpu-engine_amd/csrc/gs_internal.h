@@ -665,7 +665,7 @@ struct LossPlan {
   int32_t splits;      // shares of a piece's vocabulary in dhidden's product
   size_t stats_bytes;  // forward: a (max, sum) per row and tile
   size_t g_bytes;      // backward: a piece's gradients of the logits in bf16
-  size_t h_bytes;      // backward: H with the rows that are not scored set to zero
+  size_t h_bytes;      // backward: the hidden rows of dweight's product
   size_t part_bytes;   // backward: dhidden's shares
 };
 LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count);

@@ -1,16 +1,19 @@
 // Softmax cross entropy of the head's logits, and its gradients, without the
 // logits in memory:
 //   z = cap(H W^T),  lse[m] = log sum_v exp z[m][v],  loss[m] = lse[m] - z[m][t[m]]
-//   g[m][v] = dloss[m] (exp(z[m][v] - lse[m]) - [v = t[m]]) (1 - (z[m][v] / cap)^2)
-//   dH = g W,  dW = g^T H
+//   g[m][v] = dloss[m] / most (exp(z[m][v] - lse[m]) - [v = t[m]]) (1 - (z[m][v] / cap)^2)
+//   dH = most g W,  dW = most g^T H,  most = max |dloss|
 //
 // Four products on v_mfma_f32_16x16x32_bf16 with one main loop (tiles of 256
 // rows by kCols columns, 8 waves, 64 of the summed index a stage, operands by
 // the memory pipe straight into LDS):
 //   kStats   W x H, the epilogue leaves a (max, sum) per hidden row and tile;
 //   kGrad    W x H again, a piece of the vocabulary, the epilogue writes g in
-//            bf16 (the matrix cores read 16 bits: half a step of 2^-9 a value,
-//            sums in binary32);
+//            bf16 (the matrix cores read 16 bits: half a step of 2^-8 a value, the
+//            sums are binary32). The largest |dloss| stays out of g: where every
+//            row has the same, as in a mean, a row's largest value, at the target,
+//            is then near -1, which bf16 holds, and not a product whose rounding
+//            all rows share (dW's error at M 4096 was 1.7 times its own rounding's);
 //   kHidden  W^T x g, summed over the piece, in shares of its vocabulary rows;
 //   kWeight  H^T x g^T, summed over the hidden rows.
 // kHidden and kWeight sum over an operand's rows: those tiles lie in LDS as
@@ -25,7 +28,6 @@ namespace {
 
 enum Pass { kStats, kGrad, kHidden, kWeight };
 
-constexpr int kLossThreads = 512;
 constexpr int kRows = 256;  // rows of a tile (vocabulary rows; columns of K in kHidden and kWeight)
 constexpr int kBlock = 64;  // of the summed index a stage
 constexpr float kLog2e = 1.44269504088896341f;
@@ -45,6 +47,7 @@ struct LossArgs {
   const int32_t* targets;
   const float* lse;
   const float* dloss;
+  const float* most;   // the largest |dloss| of the scored rows
   float2* stats;       // kStats: [v_tiles][M]
   float* part;         // kHidden: [splits][M][D]
   uint16_t* dW;        // kWeight: the piece's first row
@@ -60,15 +63,20 @@ struct LossArgs {
 template <Pass kPass, int kCols>
 struct Tile {
   static constexpr bool kTrA = kPass == kHidden || kPass == kWeight, kTrB = kPass == kWeight;
-  static constexpr int kWavesR = kCols == 256 ? 2 : kCols == 128 ? 4 : 8;
-  static constexpr int kWavesC = 8 / kWavesR;
+  // 256 columns are bound by the matrix cores: 4 waves of 128 x 128, one a SIMD
+  // with the registers of two, read an LDS byte for the fewest products. Fewer
+  // columns are bound by memory: 8 waves, and more stages under way.
+  static constexpr bool kWide = kCols == 256;
+  static constexpr int kWaves = kWide ? 4 : 8, kThreads = 64 * kWaves;
+  static constexpr int kWavesR = kWide ? 2 : kCols == 128 ? 4 : 8;
+  static constexpr int kWavesC = kWaves / kWavesR;
   static constexpr int kRT = 16 / kWavesR;          // 16-row tiles a wave
   static constexpr int kCT = kCols / 16 / kWavesC;  // 16-column tiles a wave
-  static constexpr int kStages = kCols == 256 ? 2 : 3;
+  static constexpr int kStages = kWide ? 2 : 3;
   static constexpr int kA = kRows * kBlock * 2, kB = kCols * kBlock * 2;
   static constexpr int kStage = kA + kB;
-  static constexpr int kFetchB = kCols / 64;
-  static constexpr int kFetches = 4 + kFetchB;
+  static constexpr int kFetchA = 32 / kWaves, kFetchB = kCols / 8 / kWaves;  // wave instructions of 1 KB
+  static constexpr int kFetches = kFetchA + kFetchB;
   static constexpr int kOutStride = 256 + 8;        // 16-bit values a staged output row
   static constexpr int kOut = kPass == kGrad || kPass == kWeight ? kCols * kOutStride * 2 : 0;
   static constexpr int kLds = kStages * kStage > kOut ? kStages * kStage : kOut;
@@ -80,14 +88,13 @@ struct Tile {
 // different pairs of the banks.
 __device__ __forceinline__ int pair_swizzle(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-// A stage's fetches of one operand: kN wave instructions of 1 KB. `tail`: bits
-// of lanes past the last summed row (transposed operands; uniform 0 elsewhere).
+// A stage's fetches of one operand: kN wave instructions of 1 KB.
 template <int kN, typename Rsrc>
-__device__ __forceinline__ void loss_fetch(Rsrc r, char* lds, const uint32_t (&off)[kN], uint32_t k, uint32_t none) {
+__device__ __forceinline__ void loss_fetch(Rsrc r, char* lds, const uint32_t (&off)[kN], uint32_t k) {
 #ifdef __HIP_DEVICE_COMPILE__
 #pragma unroll
   for (int i = 0; i < kN; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * i), 16, off[i] | none, k, 0, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * i), 16, off[i], k, 0, 0);
 #endif
 }
 
@@ -106,17 +113,18 @@ __device__ __forceinline__ bf16x8 loss_operand(const char* p, int t, int s, uint
 #endif
 }
 
+// One stage of the narrow tiles: the next fetches go out, then two steps of 32.
 template <Pass kPass, int kCols, typename Rsrc>
 __device__ __forceinline__ void loss_block(const char* __restrict__ a, const char* __restrict__ b,
                                            char* __restrict__ a_next, char* __restrict__ b_next, Rsrc ar, Rsrc br,
-                                           const uint32_t (&a_off)[4],
+                                           const uint32_t (&a_off)[Tile<kPass, kCols>::kFetchA],
                                            const uint32_t (&b_off)[Tile<kPass, kCols>::kFetchB], uint32_t ak,
-                                           uint32_t bk, uint32_t a_none, uint32_t b_none, int a_tile, int b_tile,
-                                           const uint32_t (&a_pos)[2], const uint32_t (&b_pos)[2],
+                                           uint32_t bk, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
+                                           const uint32_t (&b_pos)[2],
                                            f32x4 (&acc)[Tile<kPass, kCols>::kRT][Tile<kPass, kCols>::kCT]) {
   typedef Tile<kPass, kCols> T;
-  loss_fetch<4>(ar, a_next, a_off, ak, a_none);
-  loss_fetch<T::kFetchB>(br, b_next, b_off, bk, b_none);
+  loss_fetch<T::kFetchA>(ar, a_next, a_off, ak);
+  loss_fetch<T::kFetchB>(br, b_next, b_off, bk);
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     bf16x8 x[T::kRT], y[T::kCT];
@@ -133,30 +141,84 @@ __device__ __forceinline__ void loss_block(const char* __restrict__ a, const cha
   }
 }
 
-// t = tanh(x / cap) of four values. Below 5/8 a polynomial (gs_cap.h), past it
-// 1 - 2 / (e^2q + 1): absolute errors near 1e-7 of the cap either way, which
-// the logarithm of the sum keeps.
-__device__ __forceinline__ void loss_tanh(const f32x4& x, float rcap, float (&t)[4]) {
-  float q[4];
-  bool small = true;
+// Half a stage of the wide tile: 64 products of the operands in registers and,
+// in a fixed order between them, the reads of the next half's operands from `a`
+// and `b` (the columns' first: every product of the next half's first eighth
+// needs them) and, in the second half, the stage's fetches. Left to the
+// compiler, the fetches go out in one run that the matrix core waits for (490
+// us for kHidden's pass at M 4096, D 2048, 32768 vocabulary rows).
+template <Pass kPass, bool kFetch, typename Rsrc>
+__device__ __forceinline__ void loss_half(const char* __restrict__ a, const char* __restrict__ b,
+                                          char* __restrict__ a_next, char* __restrict__ b_next, Rsrc ar, Rsrc br,
+                                          const uint32_t (&a_off)[8], const uint32_t (&b_off)[8], uint32_t ak,
+                                          uint32_t bk, int s, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
+                                          const uint32_t (&b_pos)[2], const bf16x8 (&x)[8], const bf16x8 (&y)[8],
+                                          bf16x8 (&x_next)[8], bf16x8 (&y_next)[8], f32x4 (&acc)[8][8]) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    q[e] = x[e] * rcap;
-    small = small && __builtin_fabsf(q[e]) < kTanhSmall;
-  }
+  for (int i = 0; i < 8; ++i) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) t[e] = tanh_small(q[e]);
-  if (!__all(small)) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float w = 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(q[e] * (2.0f * kLog2e)) + 1.0f);
-      if (!(__builtin_fabsf(q[e]) < kTanhSmall)) t[e] = w;
+    for (int h = 0; h < 4; ++h) {
+#ifdef __HIP_DEVICE_COMPILE__
+      typedef Tile<kPass, 256> T;
+      if (h < 2) {
+        const int t = 2 * (i & 3) + h;
+        if (i < 4) y_next[t] = loss_operand<T::kTrB>(b, b_tile + t, s, b_pos[0], b_pos[1]);
+        else x_next[t] = loss_operand<T::kTrA>(a, a_tile + t, s, a_pos[0], a_pos[1]);
+      } else if (kFetch) {
+        if (h == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (LdsPtr)(a_next + 1024 * i), 16, a_off[i], ak, 0, 0);
+        else __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (LdsPtr)(b_next + 1024 * i), 16, b_off[i], bk, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#endif
+      acc[i][2 * h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[2 * h], acc[i][2 * h], 0, 0, 0);
+      acc[i][2 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[2 * h + 1], acc[i][2 * h + 1], 0, 0, 0);
+#ifdef __HIP_DEVICE_COMPILE__
+      __builtin_amdgcn_sched_barrier(0);
+#endif
     }
   }
 }
 
-template <Pass kPass, int kCols>
-__global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
+// The cap, x -> cap tanh(x / cap). Below 5/8 of the cap tanh q = q (1 + s P(s)),
+// s = q^2, P of degree 4 fitted over that range (relative error 2^-27); past it
+// 1 - 2 / (e^2q + 1). Either is within 2e-7 of the cap.
+__device__ __forceinline__ float cap_series(float s) {
+  float u = -0x1.75e194p-8f;
+  u = __builtin_fmaf(u, s, 0x1.52268ep-6f);
+  u = __builtin_fmaf(u, s, -0x1.b83c58p-5f);
+  u = __builtin_fmaf(u, s, 0x1.110726p-3f);
+  u = __builtin_fmaf(u, s, -0x1.555532p-2f);
+  return __builtin_fmaf(u, s, 1.0f);
+}
+__device__ __forceinline__ float cap_far(float q) {
+  return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(q * (2.0f * kLog2e)) + 1.0f);
+}
+
+// The smallest and the largest of a lane's values of one column.
+template <int kRT, int kCT>
+__device__ __forceinline__ void column_range(const f32x4 (&acc)[kRT][kCT], int b, float& lo, float& hi) {
+  lo = __builtin_inff();
+  hi = -__builtin_inff();
+#pragma unroll
+  for (int a = 0; a < kRT; ++a) {
+    const f32x4 x = acc[a][b];
+    hi = __builtin_fmaxf(__builtin_fmaxf(hi, x[0]), x[1]);
+    hi = __builtin_fmaxf(__builtin_fmaxf(hi, x[2]), x[3]);
+    lo = __builtin_fminf(__builtin_fminf(lo, x[0]), x[1]);
+    lo = __builtin_fminf(__builtin_fminf(lo, x[2]), x[3]);
+  }
+}
+
+// A (max, sum of exponentials over it) pair with another's.
+__device__ __forceinline__ void join_sums(float& mx, float& sum, float om, float os) {
+  const float nm = __builtin_fmaxf(mx, om);
+  sum = sum * __builtin_amdgcn_exp2f((mx - nm) * kLog2e) + os * __builtin_amdgcn_exp2f((om - nm) * kLog2e);
+  mx = nm;
+}
+
+template <Pass kPass, int kCols, bool kCap>
+__global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>::kWide ? 1 : 2)) void loss_kernel(
+    LossArgs p) {
   typedef Tile<kPass, kCols> T;
   __shared__ __attribute__((aligned(16))) char lds[T::kLds];
   // An XCD (consecutive workgroups go to them in turn) takes a run of adjacent
@@ -218,23 +280,25 @@ __global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
   const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void*)B, (short)0, b_bytes, kBufferWord3);
 
   // fetch offsets and read positions. Rows of 64 (128 bytes): 16-byte chunk c of
-  // row r lands at chunk c ^ (r & 7). Transposed tiles, rows of 256 (512 bytes).
-  uint32_t a_off[4], b_off[T::kFetchB], a_pos[2], b_pos[2], rows_off[4];
+  // row r lands at chunk c ^ (r & 7). Transposed tiles: rows of 256 (512 bytes).
+  uint32_t a_off[T::kFetchA], b_off[T::kFetchB], a_pos[2], b_pos[2];
   const uint32_t nat0 = (uint32_t)(j * 128 + ((g ^ (j & 7)) * 16)), nat1 = (uint32_t)(j * 128 + (((4 + g) ^ (j & 7)) * 16));
   const uint32_t tr0 = (uint32_t)((8 * g + (j >> 2)) * 512 + (j & 3) * 8), tr1 = (uint32_t)(((j >> 2) | ((g & 1) << 2)) * 32);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) rows_off[i] = (uint32_t)(8 * wave + 2 * i + (lane >> 5));  // rows of a transposed fetch
-  auto natural = [&](int row, int stride) { return (uint32_t)(row * stride * 2 + ((lane & 7) ^ (lane >> 3)) * 16); };
+  // row of this lane in fetch i of a transposed tile (the same for both operands, where both are)
+  auto turned_row = [&](int i) __attribute__((always_inline)) { return 64 / T::kWaves * wave + 2 * i + (lane >> 5); };
+  auto natural = [&](int row, int stride) __attribute__((always_inline)) {
+    return (uint32_t)(row * stride * 2 + ((lane & 7) ^ (lane >> 3)) * 16);
+  };
   auto turned = [&](int i, int stride, int cols) __attribute__((always_inline)) {
-    const int row = (int)rows_off[i], c = (((lane & 31) >> 1) ^ pair_swizzle(row)) * 2 + (lane & 1);
+    const int row = turned_row(i), c = (((lane & 31) >> 1) ^ pair_swizzle(row)) * 2 + (lane & 1);
     return 8 * c < cols ? (uint32_t)(row * stride * 2 + c * 16) : kBufferOutOfRange;
   };
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    a_off[i] = T::kTrA ? turned(i, a_stride, D - r0) : natural(32 * wave + 8 * i + (lane >> 3), a_stride);
+  for (int i = 0; i < T::kFetchA; ++i)
+    a_off[i] = T::kTrA ? turned(i, a_stride, D - r0) : natural(kRows / T::kWaves * wave + 8 * i + (lane >> 3), a_stride);
 #pragma unroll
   for (int i = 0; i < T::kFetchB; ++i)
-    b_off[i] = T::kTrB ? turned(i, b_stride, 256) : natural(kCols / 8 * wave + 8 * i + (lane >> 3), b_stride);
+    b_off[i] = T::kTrB ? turned(i, b_stride, 256) : natural(kCols / T::kWaves * wave + 8 * i + (lane >> 3), b_stride);
   a_pos[0] = T::kTrA ? tr0 : nat0;
   a_pos[1] = T::kTrA ? tr1 : nat1;
   b_pos[0] = T::kTrB ? tr0 : nat0;
@@ -255,39 +319,72 @@ __global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
   };
   const uint32_t a_step = T::kTrA ? (uint32_t)(kBlock * a_stride * 2) : kBlock * 2;
   const uint32_t b_step = T::kTrB ? (uint32_t)(kBlock * b_stride * 2) : kBlock * 2;
-  // A block past the last is fetched as nothing (zeros); in the last block of a
-  // sum over rows, rows past it are too. (A transposed tile's eight rows of a
-  // wave: whole fetches of two rows, so the row is this lane's.)
-  auto none_of = [&](int kb, bool tr, int i) __attribute__((always_inline)) {
-    if (kb >= nk) return kBufferOutOfRange;
-    return tr && (int)at(kb) * kBlock + (int)rows_off[i] >= sums ? kBufferOutOfRange : 0u;
+  // A stage past the last is fetched as nothing (zeros); in the last stage of a
+  // sum over rows, rows past it are too.
+  auto offsets = [&](int kb, uint32_t (&ao)[T::kFetchA], uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
+    const uint32_t none = kb < nk ? 0u : kBufferOutOfRange;
+    const int rows = sums - (int)at(kb) * kBlock;
+#pragma unroll
+    for (int i = 0; i < T::kFetchA; ++i) ao[i] = a_off[i] | (T::kTrA && turned_row(i) >= rows ? kBufferOutOfRange : none);
+#pragma unroll
+    for (int i = 0; i < T::kFetchB; ++i) bo[i] = b_off[i] | (T::kTrB && turned_row(i) >= rows ? kBufferOutOfRange : none);
   };
-  auto fetch_offsets = [&](int kb, uint32_t (&ao)[4], uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ao[i] = a_off[i] | none_of(kb, T::kTrA, i);
-#pragma unroll
-    for (int i = 0; i < T::kFetchB; ++i) bo[i] = b_off[i] | none_of(kb, T::kTrB, i & 3);
+  const int a_dst = T::kA / T::kWaves * wave, b_dst = T::kA + T::kB / T::kWaves * wave;
+  const int a_tile = T::kRT * wr, b_tile = T::kCT * wc;
+  auto fetch = [&](int kb, char* stage) __attribute__((always_inline)) {
+    uint32_t ao[T::kFetchA], bo[T::kFetchB];
+    offsets(kb, ao, bo);
+    loss_fetch<T::kFetchA>(ar, stage + a_dst, ao, at(kb) * a_step);
+    loss_fetch<T::kFetchB>(br, stage + b_dst, bo, at(kb) * b_step);
   };
+  if constexpr (T::kWide) {
+    // Two buffers. A stage's operands are in registers half a stage before its
+    // last products, so its buffer is free, and the stage after next on its way
+    // into it, from the middle of a stage to the middle of the next.
+    bf16x8 x0[8], y0[8], x1[8], y1[8];
+    fetch(0, lds);
+    fetch(1, lds + T::kStage);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFetches) : "memory");
 #pragma unroll
-  for (int u = 0; u < T::kStages - 1; ++u) {
-    uint32_t ao[4], bo[T::kFetchB];
-    fetch_offsets(u, ao, bo);
-    loss_fetch<4>(ar, lds + u * T::kStage + 4096 * wave, ao, at(u) * a_step, 0);
-    loss_fetch<T::kFetchB>(br, lds + u * T::kStage + T::kA + T::kB / 8 * wave, bo, at(u) * b_step, 0);
-  }
-  for (int kb = 0; kb < nk; kb += T::kStages) {
+    for (int i = 0; i < 8; ++i) {
+      x0[i] = loss_operand<T::kTrA>(lds, a_tile + i, 0, a_pos[0], a_pos[1]);
+      y0[i] = loss_operand<T::kTrB>(lds + T::kA, b_tile + i, 0, b_pos[0], b_pos[1]);
+    }
+    for (int kb = 0; kb < nk; kb += 2) {
 #pragma unroll
-    for (int u = 0; u < T::kStages; ++u) {
-      if (kb + u < nk) {
-        // the stage has landed for every wave, and every wave has read the one before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
-        const int n = kb + u + T::kStages - 1;
-        char* next = lds + (u + T::kStages - 1) % T::kStages * T::kStage;
-        const char* cur = lds + u * T::kStage;
-        uint32_t ao[4], bo[T::kFetchB];
-        fetch_offsets(n, ao, bo);
-        loss_block<kPass, kCols>(cur, cur + T::kA, next + 4096 * wave, next + T::kA + T::kB / 8 * wave, ar, br, ao, bo,
-                                 at(n) * a_step, at(n) * b_step, 0, 0, T::kRT * wr, T::kCT * wc, a_pos, b_pos, acc);
+      for (int u = 0; u < 2; ++u) {
+        if (kb + u < nk) {
+          char* cur = lds + u * T::kStage;
+          char* other = lds + (1 - u) * T::kStage;
+          const int n = kb + u + 2;
+          uint32_t ao[8], bo[8];
+          offsets(n, ao, bo);
+          loss_half<kPass, false>(cur, cur + T::kA, nullptr, nullptr, ar, br, ao, bo, 0, 0, 1, a_tile, b_tile, a_pos,
+                                  b_pos, x0, y0, x1, y1, acc);
+          // the next stage has landed for every wave, and every wave has read this one
+          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+          loss_half<kPass, true>(other, other + T::kA, cur + a_dst, cur + b_dst, ar, br, ao, bo, at(n) * a_step,
+                                 at(n) * b_step, 0, a_tile, b_tile, a_pos, b_pos, x1, y1, x0, y0, acc);
+        }
+      }
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < T::kStages - 1; ++u) fetch(u, lds + u * T::kStage);
+    for (int kb = 0; kb < nk; kb += T::kStages) {
+#pragma unroll
+      for (int u = 0; u < T::kStages; ++u) {
+        if (kb + u < nk) {
+          // the stage has landed for every wave, and every wave has read the one before
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
+          const int n = kb + u + T::kStages - 1;
+          char* next = lds + (u + T::kStages - 1) % T::kStages * T::kStage;
+          const char* cur = lds + u * T::kStage;
+          uint32_t ao[T::kFetchA], bo[T::kFetchB];
+          offsets(n, ao, bo);
+          loss_block<kPass, kCols>(cur, cur + T::kA, next + a_dst, next + b_dst, ar, br, ao, bo, at(n) * a_step,
+                                   at(n) * b_step, a_tile, b_tile, a_pos, b_pos, acc);
+        }
       }
     }
   }
@@ -297,42 +394,58 @@ __global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
   // lane (j, g) holds rows 16 a + 4 g + e and column 16 b + j of its wave's tile
   const int row0 = 16 * T::kRT * wr + 4 * g, col0 = 16 * T::kCT * wc + j;
   if constexpr (kPass == kStats) {
-    const float rcap = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
-    float2* sums_of = (float2*)lds;  // [kWavesR][kCols]
+    const float rcap = kCap ? 1.0f / p.cap : 0.0f, rcap2 = rcap * rcap, far = kTanhSmall * p.cap;
+    const bool tail = V - r0 < kRows;  // (uniform) rows past the vocabulary count nothing
+    float2* sums_of = (float2*)lds;    // [kWavesR][kCols]
 #pragma unroll
     for (int b = 0; b < T::kCT; ++b) {
-      float mx = kLowest;
+      if (tail) {
 #pragma unroll
-      for (int a = 0; a < T::kRT; ++a) {
-        if (p.cap > 0.0f) {
-          float t[4];
-          loss_tanh(acc[a][b], rcap, t);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[a][b][e] = p.cap * t[e];
-        }
-        if (V - r0 < kRows) {  // (uniform) rows past the vocabulary count nothing
+        for (int a = 0; a < T::kRT; ++a) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (r0 + row0 + 16 * a + e >= V) acc[a][b][e] = -__builtin_inff();
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mx = __builtin_fmaxf(mx, acc[a][b][e]);
       }
-      const float ml = mx * kLog2e;
-      float sum = 0.0f;
+      float lo, mx, sum = 0.0f;
+      column_range(acc, b, lo, mx);
+      if (!kCap) {
+        mx = __builtin_fmaxf(mx, kLowest);
+        const float ml = -mx * kLog2e;
 #pragma unroll
-      for (int a = 0; a < T::kRT; ++a) {
+        for (int a = 0; a < T::kRT; ++a) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, -ml));
+          for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, ml));
+        }
+      } else {
+        const bool near = lo > -far && mx < far;  // (false with a NaN about, or a masked row)
+        mx = p.cap * cap_far(mx * rcap);          // tanh keeps the order
+        const float ml = -mx * kLog2e;
+        if (__all(near)) {
+#pragma unroll
+          for (int a = 0; a < T::kRT; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = acc[a][b][e], s = x * (x * rcap2);
+              sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x * kLog2e, cap_series(s), ml));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int a = 0; a < T::kRT; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = acc[a][b][e], q = x * rcap;
+              const float z = __builtin_fabsf(q) < kTanhSmall ? x * cap_series(q * q) : p.cap * cap_far(q);
+              const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, ml));
+              sum += tail && r0 + row0 + 16 * a + e >= V ? 0.0f : v;
+            }
+          }
+        }
       }
       // the four lane groups of a column
 #pragma unroll
-      for (int d = 16; d < 64; d <<= 1) {
-        const float om = __shfl_xor(mx, d), os = __shfl_xor(sum, d);
-        const float nm = __builtin_fmaxf(mx, om);
-        sum = sum * __builtin_amdgcn_exp2f((mx - nm) * kLog2e) + os * __builtin_amdgcn_exp2f((om - nm) * kLog2e);
-        mx = nm;
-      }
+      for (int d = 16; d < 64; d <<= 1) join_sums(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
       if (g == 0) sums_of[wr * kCols + col0 + 16 * b] = make_float2(mx, sum);
     }
     __syncthreads();
@@ -341,63 +454,69 @@ __global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
 #pragma unroll
       for (int w = 1; w < T::kWavesR; ++w) {
         const float2 o = sums_of[w * kCols + tid];
-        const float nm = __builtin_fmaxf(s.x, o.x);
-        s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
-        s.x = nm;
+        join_sums(s.x, s.y, o.x, o.y);
       }
       p.stats[(size_t)rt * M + c0 + tid] = s;
     }
   } else if constexpr (kPass == kGrad) {
-    const float rcap = p.cap > 0.0f ? 1.0f / p.cap : 0.0f;
+    const float rcap = kCap ? 1.0f / p.cap : 0.0f, rcap2 = rcap * rcap, far = kTanhSmall * p.cap;
     uint16_t* stage = (uint16_t*)lds;
 #pragma unroll
     for (int b = 0; b < T::kCT; ++b) {
       const int col = col0 + 16 * b, m = c0 + col;
       const int target = m < M ? p.targets[m] : -1;
       const bool scored = target >= 0 && target < p.vocab;
-      const float ll = m < M ? p.lse[m] * kLog2e : 0.0f;
-      const float d = m < M ? p.dloss[m] : 0.0f;
+      const float ll = m < M ? -p.lse[m] * kLog2e : 0.0f;
+      const float most = *p.most, share = m < M && most > 0.0f ? p.dloss[m] / most : most;
       const int hit = target - p.v_base - r0 - row0;  // the target's place among this lane's rows
-      const bool any_hit = __any(target >= 0 && hit >= 0 && hit < 16 * T::kRT);
+      const bool any_hit = __any(scored && hit >= 0 && hit < 16 * T::kRT);
+      bool near = true;
+      if (kCap) {
+        float lo, hi;
+        column_range(acc, b, lo, hi);
+        near = __all(lo > -far && hi < far);
+      }
 #pragma unroll
       for (int a = 0; a < T::kRT; ++a) {
-        float v[4], t[4];
-        if (p.cap > 0.0f) {
-          loss_tanh(acc[a][b], rcap, t);
+        float v[4], w[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = p.cap * t[e];
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = acc[a][b][e];
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc[a][b][e];
+          w[e] = 1.0f;
+          if (!kCap) {
+            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, ll));
+          } else if (near) {
+            const float s = x * (x * rcap2), u = cap_series(s);
+            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x * kLog2e, u, ll));
+            w[e] = __builtin_fmaf(-s, u * u, 1.0f);
+          } else {
+            const float q = x * rcap;
+            const float t = __builtin_fabsf(q) < kTanhSmall ? q * cap_series(q * q) : cap_far(q);
+            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p.cap * t, kLog2e, ll));
+            w[e] = __builtin_fmaf(-t, t, 1.0f);
+          }
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(v[e], kLog2e, -ll));
         if (any_hit) {  // (uniform)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (hit == 16 * a + e) v[e] -= 1.0f;
         }
-        if (p.cap > 0.0f) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= d * __builtin_fmaf(-t[e], t[e], 1.0f);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] *= d;
-        }
+        for (int e = 0; e < 4; ++e) v[e] *= kCap ? w[e] * share : share;
         if (V - r0 < kRows) {  // (uniform) zeros past the vocabulary
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (r0 + row0 + 16 * a + e >= V) v[e] = 0.0f;
         }
         // a row that is not scored has no gradient, whatever its hidden state holds
-        const MxU32x2 w = {scored ? pack_bf16(v[0], v[1]) : 0u, scored ? pack_bf16(v[2], v[3]) : 0u};
-        *(MxU32x2*)&stage[col * T::kOutStride + row0 + 16 * a] = w;
+        const MxU32x2 o = {scored ? pack_bf16(v[0], v[1]) : 0u, scored ? pack_bf16(v[2], v[3]) : 0u};
+        *(MxU32x2*)&stage[col * T::kOutStride + row0 + 16 * a] = o;
       }
     }
     __syncthreads();
     // rows of 512 bytes of g
 #pragma unroll 4
-    for (int q = tid; q < kCols * 32; q += kLossThreads) {
+    for (int q = tid; q < kCols * 32; q += T::kThreads) {
       const int m = q >> 5, c = (q & 31) * 8;
       if (c0 + m < M)
         *(MxU32x4*)&p.G[(size_t)(c0 + m) * p.g_stride + r0 + c] = *(const MxU32x4*)&stage[m * T::kOutStride + c];
@@ -420,18 +539,19 @@ __global__ __launch_bounds__(kLossThreads, 2) void loss_kernel(LossArgs p) {
     }
   } else {
     uint16_t* stage = (uint16_t*)lds;
+    const float most = *p.most;
 #pragma unroll
     for (int b = 0; b < T::kCT; ++b) {
 #pragma unroll
       for (int a = 0; a < T::kRT; ++a) {
-        const f32x4 v = acc[a][b];
+        const f32x4 v = acc[a][b] * most;
         *(MxU32x2*)&stage[(col0 + 16 * b) * T::kOutStride + row0 + 16 * a] =
             MxU32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
       }
     }
     __syncthreads();
 #pragma unroll 4
-    for (int q = tid; q < kCols * 32; q += kLossThreads) {
+    for (int q = tid; q < kCols * 32; q += T::kThreads) {
       const int v = q >> 5, c = (q & 31) * 8;
       if (c0 + v < V && r0 + c < D)
         *(MxU32x4*)&p.dW[(size_t)(c0 + v) * D + r0 + c] = *(const MxU32x4*)&stage[v * T::kOutStride + c];
@@ -455,9 +575,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict
 #pragma unroll 4
     for (int t = slice; t < n_tiles; t += 32) {
       const float2 o = stats[(size_t)t * M + m0 + i];
-      const float nm = __builtin_fmaxf(s.x, o.x);
-      s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
-      s.x = nm;
+      join_sums(s.x, s.y, o.x, o.y);
     }
   }
   slices[slice][i] = s;
@@ -465,9 +583,7 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict
   if (slice == 0 && m0 + i < M) {
     for (int t = 1; t < 32; ++t) {
       const float2 o = slices[t][i];
-      const float nm = __builtin_fmaxf(s.x, o.x);
-      s.y = s.y * __builtin_amdgcn_exp2f((s.x - nm) * kLog2e) + o.y * __builtin_amdgcn_exp2f((o.x - nm) * kLog2e);
-      s.x = nm;
+      join_sums(s.x, s.y, o.x, o.y);
     }
     const float l = s.x + logf(s.y);
     lse_of[i] = l;
@@ -496,8 +612,33 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict
   }
 }
 
-// H with zeros in the rows that are not scored, for dW's product (their g is
-// zero, but zero times what a padded row may hold need not be).
+// The largest |dloss| of the scored rows (a NaN stays one: its bits are above
+// every number's).
+__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* __restrict__ dloss,
+                                                          const int32_t* __restrict__ targets, int M, int V,
+                                                          float* __restrict__ most) {
+  __shared__ uint32_t wave_most[16];
+  uint32_t b = 0;
+  for (int m = threadIdx.x; m < M; m += 1024) {
+    const int t = targets[m];
+    const uint32_t d = t >= 0 && t < V ? __float_as_uint(dloss[m]) & 0x7fffffffu : 0u;
+    b = d > b ? d : b;
+  }
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)b, d);
+    b = o > b ? o : b;
+  }
+  if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = b;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 16; ++i) b = wave_most[i] > b ? wave_most[i] : b;
+    *most = __uint_as_float(b);
+  }
+}
+
+// H with zeros in the rows that are not scored, for dW's product: their g is
+// zero, but zero times what a padded row may hold need not be.
 __global__ __launch_bounds__(256) void loss_rows_kernel(const uint16_t* __restrict__ H,
                                                         const int32_t* __restrict__ targets, int V, int D, int64_t n,
                                                         uint16_t* __restrict__ out) {
@@ -508,35 +649,56 @@ __global__ __launch_bounds__(256) void loss_rows_kernel(const uint16_t* __restri
   *(MxU32x4*)&out[e] = t >= 0 && t < V ? *(const MxU32x4*)&H[e] : z;
 }
 
-// dH = the shares, added in order and rounded once.
+// dH = most times the shares, added in order and rounded once; zeros in the rows
+// that are not scored.
 __global__ __launch_bounds__(256) void loss_hidden_kernel(const float* __restrict__ part, int splits, int64_t n,
+                                                          const int32_t* __restrict__ targets,
+                                                          const float* __restrict__ most, int V, int D,
                                                           uint16_t* __restrict__ dH) {
   const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
   if (e >= n) return;
+  const int t = targets[e / D];
   float v[8];
   load_8<false>(part, e, 8, v);
+#pragma unroll 4
   for (int s = 1; s < splits; ++s) {
     float o[8];
     load_8<false>(part, s * n + e, 8, o);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += o[i];
   }
+  const float f = *most;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = t >= 0 && t < V ? v[i] * f : 0.0f;
   store_8<true>(dH, e, 8, v);
+}
+
+template <Pass kPass, bool kCap>
+void loss_launch_capped(const LossArgs& p, int cols, hipStream_t s) {
+  const int total = p.row_tiles * p.col_tiles * p.splits;
+  const dim3 grid((unsigned)((total + 7) / 8 * 8));
+  if constexpr (kPass != kWeight) {
+    if (cols == 64) {
+      loss_kernel<kPass, 64, kCap><<<grid, dim3(Tile<kPass, 64>::kThreads), 0, s>>>(p);
+      return;
+    }
+    if (cols == 128) {
+      loss_kernel<kPass, 128, kCap><<<grid, dim3(Tile<kPass, 128>::kThreads), 0, s>>>(p);
+      return;
+    }
+  }
+  loss_kernel<kPass, 256, kCap><<<grid, dim3(Tile<kPass, 256>::kThreads), 0, s>>>(p);
 }
 
 template <Pass kPass>
 void loss_launch(const LossArgs& p, int cols, hipStream_t s) {
-  const int total = p.row_tiles * p.col_tiles * p.splits;
-  const dim3 grid((unsigned)((total + 7) / 8 * 8)), block(kLossThreads);
-  if constexpr (kPass == kWeight) {
-    loss_kernel<kPass, 256><<<grid, block, 0, s>>>(p);
-  } else if (cols == 64) {
-    loss_kernel<kPass, 64><<<grid, block, 0, s>>>(p);
-  } else if (cols == 128) {
-    loss_kernel<kPass, 128><<<grid, block, 0, s>>>(p);
-  } else {
-    loss_kernel<kPass, 256><<<grid, block, 0, s>>>(p);
+  if constexpr (kPass == kStats || kPass == kGrad) {
+    if (p.cap > 0.0f) {
+      loss_launch_capped<kPass, true>(p, cols, s);
+      return;
+    }
   }
+  loss_launch_capped<kPass, false>(p, cols, s);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -588,6 +750,8 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
   const dim3 per8((unsigned)((n / 8 + 255) / 256)), block(256);
   uint16_t* scored = (uint16_t*)(work + plan.g_bytes);
   float* part = (float*)(work + plan.g_bytes + plan.h_bytes);
+  float* most = (float*)(work + plan.g_bytes + plan.h_bytes + plan.part_bytes);
+  loss_scale_kernel<<<dim3(1), dim3(1024), 0, s>>>(dloss, targets, rows, vocab, most);
   if (dweight) loss_rows_kernel<<<per8, block, 0, s>>>(hidden, targets, vocab, width, n, scored);
   const int k_tiles = (width + kRows - 1) / kRows;
   int splits = 1;
@@ -599,6 +763,7 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
     p.targets = targets;
     p.lse = lse;
     p.dloss = dloss;
+    p.most = most;
     p.part = part;
     p.cap = softcap;
     p.M = rows;
@@ -629,7 +794,7 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
       loss_launch<kWeight>(p, 256, s);
     }
   }
-  if (dhidden) loss_hidden_kernel<<<per8, block, 0, s>>>(part, splits, n, dhidden);
+  if (dhidden) loss_hidden_kernel<<<per8, block, 0, s>>>(part, splits, n, targets, most, vocab, width, dhidden);
 }
 
 }  // namespace gs
