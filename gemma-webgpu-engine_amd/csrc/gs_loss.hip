@@ -60,6 +60,12 @@ struct LossArgs {
   int32_t accumulate;  // kHidden: add to the shares of the pieces before
 };
 
+struct Column {
+  int32_t target;  // negative: not scored
+  float ll;        // -lse log2(e)
+  float share;     // dloss over the largest |dloss|
+};
+
 template <Pass kPass, int kCols>
 struct Tile {
   static constexpr bool kTrA = kPass == kHidden || kPass == kWeight, kTrB = kPass == kWeight;
@@ -79,7 +85,9 @@ struct Tile {
   static constexpr int kFetches = kFetchA + kFetchB;
   static constexpr int kOutStride = 256 + 8;        // 16-bit values a staged output row
   static constexpr int kOut = kPass == kGrad || kPass == kWeight ? kCols * kOutStride * 2 : 0;
-  static constexpr int kLds = kStages * kStage > kOut ? kStages * kStage : kOut;
+  static constexpr int kOperands = kWide ? 5 * kA : kStages * kStage;  // (kWide: kA == kB)
+  static constexpr int kColumns = kPass == kGrad ? kCols * (int)sizeof(Column) : 0;
+  static constexpr int kLds = kOperands > kOut + kColumns ? kOperands : kOut + kColumns;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
 
@@ -144,14 +152,14 @@ __device__ __forceinline__ void loss_block(const char* __restrict__ a, const cha
 // Half a stage of the wide tile: 64 products of the operands in registers and,
 // in a fixed order between them, the reads of the next half's operands from `a`
 // and `b` (the columns' first: every product of the next half's first eighth
-// needs them) and, in the second half, the stage's fetches. Left to the
-// compiler, the fetches go out in one run that the matrix core waits for (490
-// us for kHidden's pass at M 4096, D 2048, 32768 vocabulary rows).
-template <Pass kPass, bool kFetch, typename Rsrc>
+// needs them) and the fetches of one operand's tile of a later stage (kSlots of
+// the 16 places for them). Left to the compiler, the fetches go out in one run
+// that the matrix core waits for (dH's product at M 4096, D 2048, 32768
+// vocabulary rows took 490 us).
+template <Pass kPass, int kSlots, typename Rsrc>
 __device__ __forceinline__ void loss_half(const char* __restrict__ a, const char* __restrict__ b,
-                                          char* __restrict__ a_next, char* __restrict__ b_next, Rsrc ar, Rsrc br,
-                                          const uint32_t (&a_off)[8], const uint32_t (&b_off)[8], uint32_t ak,
-                                          uint32_t bk, int s, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
+                                          char* __restrict__ next, Rsrc rsrc, const uint32_t (&off)[8], uint32_t k,
+                                          int s, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
                                           const uint32_t (&b_pos)[2], const bf16x8 (&x)[8], const bf16x8 (&y)[8],
                                           bf16x8 (&x_next)[8], bf16x8 (&y_next)[8], f32x4 (&acc)[8][8]) {
 #pragma unroll
@@ -164,9 +172,10 @@ __device__ __forceinline__ void loss_half(const char* __restrict__ a, const char
         const int t = 2 * (i & 3) + h;
         if (i < 4) y_next[t] = loss_operand<T::kTrB>(b, b_tile + t, s, b_pos[0], b_pos[1]);
         else x_next[t] = loss_operand<T::kTrA>(a, a_tile + t, s, a_pos[0], a_pos[1]);
-      } else if (kFetch) {
-        if (h == 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (LdsPtr)(a_next + 1024 * i), 16, a_off[i], ak, 0, 0);
-        else __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (LdsPtr)(b_next + 1024 * i), 16, b_off[i], bk, 0, 0);
+      } else {
+        const int slot = 2 * i + h - 2, n = slot * 8 / kSlots;
+        if (n < 8 && slot * 8 % kSlots == 0)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(next + 1024 * n), 16, off[n], k, 0, 0);
       }
       __builtin_amdgcn_sched_barrier(0);
 #endif
@@ -246,6 +255,16 @@ __global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>
   const int M = p.M, D = p.D, V = p.V;
   const int r0 = rt * kRows, c0 = ct * kCols;
 
+  // kGrad: what the epilogue needs of column tid, read now and kept
+  Column column{-1, 0.0f, 0.0f};
+  if (kPass == kGrad && tid < kCols && c0 + tid < M) {
+    const int t = p.targets[c0 + tid];
+    const float most = *p.most;
+    column.target = t < p.vocab ? t : -1;
+    column.ll = -p.lse[c0 + tid] * kLog2e;
+    column.share = most > 0.0f ? p.dloss[c0 + tid] / most : most;
+  }
+
   // operands: where their first row lies, how many rows there are, their stride
   const int sum0 = kPass == kHidden ? split * p.split_rows : 0;  // first of the summed index
   int sums = kPass == kHidden ? (V - sum0 < p.split_rows ? V - sum0 : p.split_rows) : kPass == kWeight ? M : D;
@@ -321,56 +340,67 @@ __global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>
   const uint32_t b_step = T::kTrB ? (uint32_t)(kBlock * b_stride * 2) : kBlock * 2;
   // A stage past the last is fetched as nothing (zeros); in the last stage of a
   // sum over rows, rows past it are too.
-  auto offsets = [&](int kb, uint32_t (&ao)[T::kFetchA], uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
+  auto offsets_a = [&](int kb, uint32_t (&ao)[T::kFetchA]) __attribute__((always_inline)) {
     const uint32_t none = kb < nk ? 0u : kBufferOutOfRange;
     const int rows = sums - (int)at(kb) * kBlock;
 #pragma unroll
     for (int i = 0; i < T::kFetchA; ++i) ao[i] = a_off[i] | (T::kTrA && turned_row(i) >= rows ? kBufferOutOfRange : none);
+  };
+  auto offsets_b = [&](int kb, uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
+    const uint32_t none = kb < nk ? 0u : kBufferOutOfRange;
+    const int rows = sums - (int)at(kb) * kBlock;
 #pragma unroll
     for (int i = 0; i < T::kFetchB; ++i) bo[i] = b_off[i] | (T::kTrB && turned_row(i) >= rows ? kBufferOutOfRange : none);
   };
-  const int a_dst = T::kA / T::kWaves * wave, b_dst = T::kA + T::kB / T::kWaves * wave;
+  const int a_dst = T::kA / T::kWaves * wave, b_dst = T::kB / T::kWaves * wave;
   const int a_tile = T::kRT * wr, b_tile = T::kCT * wc;
-  auto fetch = [&](int kb, char* stage) __attribute__((always_inline)) {
+  auto fetch = [&](int kb, char* a, char* b) __attribute__((always_inline)) {
     uint32_t ao[T::kFetchA], bo[T::kFetchB];
-    offsets(kb, ao, bo);
-    loss_fetch<T::kFetchA>(ar, stage + a_dst, ao, at(kb) * a_step);
-    loss_fetch<T::kFetchB>(br, stage + b_dst, bo, at(kb) * b_step);
+    offsets_a(kb, ao);
+    offsets_b(kb, bo);
+    loss_fetch<T::kFetchA>(ar, a + a_dst, ao, at(kb) * a_step);
+    loss_fetch<T::kFetchB>(br, b + b_dst, bo, at(kb) * b_step);
   };
   if constexpr (T::kWide) {
-    // Two buffers. A stage's operands are in registers half a stage before its
-    // last products, so its buffer is free, and the stage after next on its way
-    // into it, from the middle of a stage to the middle of the next.
+    // The stages' tiles (A, B, A, B, ...) take five places in turn. A stage's
+    // operands are in registers half a stage before its last products, so from
+    // the middle of stage k on its two places are free: B of stage k + 2 is
+    // fetched into the one in the second half (early in it), A of stage k + 3
+    // into the other in the next stage's first half, and both have landed by the
+    // middle of the stage before theirs. (All fetches in the second half, into
+    // two whole buffers, took 3% more.)
     bf16x8 x0[8], y0[8], x1[8], y1[8];
-    fetch(0, lds);
-    fetch(1, lds + T::kStage);
+    fetch(0, lds, lds + T::kA);
+    fetch(1, lds + 2 * T::kA, lds + 3 * T::kA);
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFetches) : "memory");
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       x0[i] = loss_operand<T::kTrA>(lds, a_tile + i, 0, a_pos[0], a_pos[1]);
       y0[i] = loss_operand<T::kTrB>(lds + T::kA, b_tile + i, 0, b_pos[0], b_pos[1]);
     }
-    for (int kb = 0; kb < nk; kb += 2) {
+    for (int kb = 0; kb < nk; kb += 5) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < 5; ++u) {
         if (kb + u < nk) {
-          char* cur = lds + u * T::kStage;
-          char* other = lds + (1 - u) * T::kStage;
+          const char *a = lds + 2 * u % 5 * T::kA, *b = lds + (2 * u + 1) % 5 * T::kA;
+          const char *a1 = lds + (2 * u + 2) % 5 * T::kA, *b1 = lds + (2 * u + 3) % 5 * T::kA;
+          char *a2 = lds + (2 * u + 4) % 5 * T::kA, *b2 = lds + 2 * u % 5 * T::kA;
           const int n = kb + u + 2;
-          uint32_t ao[8], bo[8];
-          offsets(n, ao, bo);
-          loss_half<kPass, false>(cur, cur + T::kA, nullptr, nullptr, ar, br, ao, bo, 0, 0, 1, a_tile, b_tile, a_pos,
-                                  b_pos, x0, y0, x1, y1, acc);
+          uint32_t off[8];
+          offsets_a(n, off);
+          loss_half<kPass, 16>(a, b, a2 + a_dst, ar, off, at(n) * a_step, 1, a_tile, b_tile, a_pos, b_pos, x0, y0, x1,
+                               y1, acc);
           // the next stage has landed for every wave, and every wave has read this one
-          asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-          loss_half<kPass, true>(other, other + T::kA, cur + a_dst, cur + b_dst, ar, br, ao, bo, at(n) * a_step,
-                                 at(n) * b_step, 0, a_tile, b_tile, a_pos, b_pos, x1, y1, x0, y0, acc);
+          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kFetchA) : "memory");
+          offsets_b(n, off);
+          loss_half<kPass, 8>(a1, b1, b2 + b_dst, br, off, at(n) * b_step, 0, a_tile, b_tile, a_pos, b_pos, x1, y1, x0,
+                              y0, acc);
         }
       }
     }
   } else {
 #pragma unroll
-    for (int u = 0; u < T::kStages - 1; ++u) fetch(u, lds + u * T::kStage);
+    for (int u = 0; u < T::kStages - 1; ++u) fetch(u, lds + u * T::kStage, lds + u * T::kStage + T::kA);
     for (int kb = 0; kb < nk; kb += T::kStages) {
 #pragma unroll
       for (int u = 0; u < T::kStages; ++u) {
@@ -381,8 +411,9 @@ __global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>
           char* next = lds + (u + T::kStages - 1) % T::kStages * T::kStage;
           const char* cur = lds + u * T::kStage;
           uint32_t ao[T::kFetchA], bo[T::kFetchB];
-          offsets(n, ao, bo);
-          loss_block<kPass, kCols>(cur, cur + T::kA, next + a_dst, next + b_dst, ar, br, ao, bo, at(n) * a_step,
+          offsets_a(n, ao);
+          offsets_b(n, bo);
+          loss_block<kPass, kCols>(cur, cur + T::kA, next + a_dst, next + T::kA + b_dst, ar, br, ao, bo, at(n) * a_step,
                                    at(n) * b_step, a_tile, b_tile, a_pos, b_pos, acc);
         }
       }
@@ -391,6 +422,11 @@ __global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>
   // nothing is in flight to or from LDS before the epilogue uses it
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 
+  if constexpr (kPass == kGrad) {
+    // the columns' values behind the staged outputs
+    if (tid < kCols) ((Column*)(lds + T::kOut))[tid] = column;
+    __syncthreads();
+  }
   // lane (j, g) holds rows 16 a + 4 g + e and column 16 b + j of its wave's tile
   const int row0 = 16 * T::kRT * wr + 4 * g, col0 = 16 * T::kCT * wc + j;
   if constexpr (kPass == kStats) {
@@ -463,12 +499,11 @@ __global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>
     uint16_t* stage = (uint16_t*)lds;
 #pragma unroll
     for (int b = 0; b < T::kCT; ++b) {
-      const int col = col0 + 16 * b, m = c0 + col;
-      const int target = m < M ? p.targets[m] : -1;
-      const bool scored = target >= 0 && target < p.vocab;
-      const float ll = m < M ? -p.lse[m] * kLog2e : 0.0f;
-      const float most = *p.most, share = m < M && most > 0.0f ? p.dloss[m] / most : most;
-      const int hit = target - p.v_base - r0 - row0;  // the target's place among this lane's rows
+      const int col = col0 + 16 * b;
+      const Column c = ((const Column*)(lds + T::kOut))[col];
+      const bool scored = c.target >= 0;
+      const float ll = c.ll, share = c.share;
+      const int hit = c.target - p.v_base - r0 - row0;  // the target's place among this lane's rows
       const bool any_hit = __any(scored && hit >= 0 && hit < 16 * T::kRT);
       bool near = true;
       if (kCap) {
