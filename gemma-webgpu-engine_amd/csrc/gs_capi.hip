@@ -1373,7 +1373,7 @@ int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight,
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "targets, lse and dloss must be aligned to their elements");
   GS_HIP(ctx, hipSetDevice(ctx->device));
   const LossPlan plan = loss_plan(rows, width, ctx->vocab, ctx->cu_count);
-  st = ensure_work(ctx, plan.g_bytes + plan.h_bytes + plan.part_bytes + 256, s);
+  st = ensure_work(ctx, plan.g_bytes + plan.h_bytes + plan.part_bytes + 256 + (size_t)rows * 16, s);
   if (st != GS_OK) return st;
   launch_lmhead_loss_grad((const uint16_t*)hidden, (const uint16_t*)weight, targets, lse, dloss, rows, width, ctx->vocab,
                           softcap, plan, ctx->d_work, (uint16_t*)dhidden, (uint16_t*)dweight, s);

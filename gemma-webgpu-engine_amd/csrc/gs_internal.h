@@ -659,7 +659,8 @@ void launch_mx_lmhead(const uint8_t* hidden, const uint8_t* hidden_scales, const
 
 // ------------------------------------------- the head's cross entropy
 struct LossPlan {
-  int32_t cols;        // rows of H in a tile: 64, 128 or 256
+  int32_t cols;        // rows of H in a tile: 64, 128, 160, 192 or 256
+  int32_t cus;         // compute units
   int32_t v_tiles;     // tiles of 256 vocabulary rows
   int32_t piece;       // vocabulary rows whose gradients are held at a time, a multiple of 256
   int32_t splits;      // shares of a piece's vocabulary in dhidden's product

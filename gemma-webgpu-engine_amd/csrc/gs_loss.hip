@@ -4,9 +4,12 @@
 //   g[m][v] = dloss[m] / most (exp(z[m][v] - lse[m]) - [v = t[m]]) (1 - (z[m][v] / cap)^2)
 //   dH = most g W,  dW = most g^T H,  most = max |dloss|
 //
-// Four products on v_mfma_f32_16x16x32_bf16 with one main loop (tiles of 256
-// rows by kCols columns, 8 waves, 64 of the summed index a stage, operands by
-// the memory pipe straight into LDS):
+// Four products on v_mfma_f32_16x16x32_bf16 with one main loop: tiles of 256
+// rows by kCols columns, 4 waves of 128 by kCols / 2, one a SIMD with the
+// registers of two (an LDS byte is read for the fewest products so), 64 of the
+// summed index a stage, operands by the memory pipe straight into LDS. A
+// workgroup takes tile after tile and fetches the next one's first stages while
+// it finishes the last.
 //   kStats   W x H, the epilogue leaves a (max, sum) per hidden row and tile;
 //   kGrad    W x H again, a piece of the vocabulary, the epilogue writes g in
 //            bf16 (the matrix cores read 16 bits: half a step of 2^-8 a value, the
@@ -28,6 +31,7 @@ namespace {
 
 enum Pass { kStats, kGrad, kHidden, kWeight };
 
+constexpr int kLossThreads = 256;
 constexpr int kRows = 256;  // rows of a tile (vocabulary rows; columns of K in kHidden and kWeight)
 constexpr int kBlock = 64;  // of the summed index a stage
 constexpr float kLog2e = 1.44269504088896341f;
@@ -40,54 +44,49 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void* LdsPtr;
 typedef __attribute__((address_space(3))) i16x4* LdsTrPtr;
 
-struct LossArgs {
-  const uint16_t* W;   // the piece's first row
-  const uint16_t* H;
-  uint16_t* G;         // [M][g_stride]
-  const int32_t* targets;
-  const float* lse;
-  const float* dloss;
-  const float* most;   // the largest |dloss| of the scored rows
-  float2* stats;       // kStats: [v_tiles][M]
-  float* part;         // kHidden: [splits][M][D]
-  uint16_t* dW;        // kWeight: the piece's first row
-  float cap;
-  int32_t M, D, V;     // V: vocabulary rows of the piece
-  int32_t v_base;      // the piece's first vocabulary row
-  int32_t vocab;
-  int32_t g_stride;    // a multiple of 256, at least V
-  int32_t row_tiles, col_tiles, splits, split_rows;  // split_rows: vocabulary rows a share, a multiple of 64
-  int32_t accumulate;  // kHidden: add to the shares of the pieces before
-};
-
+// What kGrad needs of a hidden row.
 struct Column {
   int32_t target;  // negative: not scored
   float ll;        // -lse log2(e)
   float share;     // dloss over the largest |dloss|
+  float none;
+};
+
+struct LossArgs {
+  const uint16_t* W;      // the piece's first row
+  const uint16_t* H;
+  uint16_t* G;            // [M][g_stride]
+  const Column* columns;  // [M]
+  const float* most;      // the largest |dloss| of the scored rows
+  float2* stats;          // kStats: [v_tiles][M]
+  float* part;            // kHidden: [splits][M][D]
+  uint16_t* dW;           // kWeight: the piece's first row
+  float cap;
+  int32_t M, D, V;        // V: vocabulary rows of the piece
+  int32_t v_base;         // the piece's first vocabulary row
+  int32_t g_stride;       // a multiple of 256, at least V
+  int32_t row_tiles, col_tiles, splits, split_rows;  // split_rows: vocabulary rows a share, a multiple of 64
+  int32_t accumulate;     // kHidden: add to the shares of the pieces before
 };
 
 template <Pass kPass, int kCols>
 struct Tile {
   static constexpr bool kTrA = kPass == kHidden || kPass == kWeight, kTrB = kPass == kWeight;
-  // 256 columns are bound by the matrix cores: 4 waves of 128 x 128, one a SIMD
-  // with the registers of two, read an LDS byte for the fewest products. Fewer
-  // columns are bound by memory: 8 waves, and more stages under way.
-  static constexpr bool kWide = kCols == 256;
-  static constexpr int kWaves = kWide ? 4 : 8, kThreads = 64 * kWaves;
-  static constexpr int kWavesR = kWide ? 2 : kCols == 128 ? 4 : 8;
-  static constexpr int kWavesC = kWaves / kWavesR;
-  static constexpr int kRT = 16 / kWavesR;          // 16-row tiles a wave
-  static constexpr int kCT = kCols / 16 / kWavesC;  // 16-column tiles a wave
-  static constexpr int kStages = kWide ? 2 : 3;
+  static constexpr int kCT = kCols / 32;     // 16-column tiles a wave (two waves abreast)
   static constexpr int kA = kRows * kBlock * 2, kB = kCols * kBlock * 2;
-  static constexpr int kStage = kA + kB;
-  static constexpr int kFetchA = 32 / kWaves, kFetchB = kCols / 8 / kWaves;  // wave instructions of 1 KB
-  static constexpr int kFetches = kFetchA + kFetchB;
-  static constexpr int kOutStride = 256 + 8;        // 16-bit values a staged output row
-  static constexpr int kOut = kPass == kGrad || kPass == kWeight ? kCols * kOutStride * 2 : 0;
-  static constexpr int kOperands = kWide ? 5 * kA : kStages * kStage;  // (kWide: kA == kB)
-  static constexpr int kColumns = kPass == kGrad ? kCols * (int)sizeof(Column) : 0;
-  static constexpr int kLds = kOperands > kOut + kColumns ? kOperands : kOut + kColumns;
+  static constexpr int kFetchB = kCT;        // wave instructions of 1 KB (8 for the rows)
+  // Wide tiles: the stages' tiles (A, B, A, B, ...) take five places of 32 KB in
+  // turn, two stages ahead. Narrow ones: whole stages in three places, three ahead.
+  static constexpr bool kFive = kCols >= 192;
+  static constexpr int kPlace = kFive ? kA : kA + kB;
+  static constexpr int kScratch = 4096;      // a (max, sum) a row half and column, or the columns' values
+  static constexpr int kOperands = kFive ? 5 * kA : 3 * kPlace;
+  static constexpr int kLds = kFive ? kOperands : kOperands + kScratch;
+  // fetches after the next stage's own when that one has to have landed
+  static constexpr int kAhead = kFive ? 8 : 8 + kFetchB;
+  // stores of a tile's epilogue, always issued, that may still be under way then
+  static constexpr int kStores = kPass == kStats ? 0 : kPass == kHidden ? 8 * kCT : 4 * kCT;
+  static constexpr int kAheadStores = kAhead + kStores < 63 ? kAhead + kStores : 63;
   static_assert(kLds <= 160 * 1024, "LDS of a compute unit");
 };
 
@@ -96,23 +95,14 @@ struct Tile {
 // different pairs of the banks.
 __device__ __forceinline__ int pair_swizzle(int row) { return (row & 3) | ((row >> 1) & 4); }
 
-// A stage's fetches of one operand: kN wave instructions of 1 KB.
-template <int kN, typename Rsrc>
-__device__ __forceinline__ void loss_fetch(Rsrc r, char* lds, const uint32_t (&off)[kN], uint32_t k) {
-#ifdef __HIP_DEVICE_COMPILE__
-#pragma unroll
-  for (int i = 0; i < kN; ++i)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * i), 16, off[i], k, 0, 0);
-#endif
-}
-
-// Operand tile t's values of the summed index 32 s + 8 g .. + 7 for lane (j, g).
+// Operand tile t's values of the summed index 32 s + 8 g .. + 7 for lane (j, g),
+// from the wave's first tile. Rows of 64: pos is the lane's row and chunk.
+// Transposed: its row and place in a pair, turn the pair's swizzle.
 template <bool kTr>
-__device__ __forceinline__ bf16x8 loss_operand(const char* p, int t, int s, uint32_t pos0, uint32_t pos1) {
-  if (!kTr) return *(const bf16x8*)(p + 2048 * t + (s ? pos1 : pos0));
+__device__ __forceinline__ bf16x8 loss_operand(const char* p, int t, int s, uint32_t pos, uint32_t turn) {
+  if (!kTr) return *(const bf16x8*)(p + pos + 2048 * t);
 #ifdef __HIP_DEVICE_COMPILE__
-  // pos0: this lane's row and place in a pair, pos1: its swizzle
-  const char* q = p + s * 16384 + pos0 + ((32 * (uint32_t)t) ^ pos1);
+  const char* q = p + pos + ((32 * (uint32_t)t) ^ turn) + s * 16384;
   const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTrPtr)q);
   const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsTrPtr)(q + 2048));
   return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -121,102 +111,160 @@ __device__ __forceinline__ bf16x8 loss_operand(const char* p, int t, int s, uint
 #endif
 }
 
-// One stage of the narrow tiles: the next fetches go out, then two steps of 32.
-template <Pass kPass, int kCols, typename Rsrc>
-__device__ __forceinline__ void loss_block(const char* __restrict__ a, const char* __restrict__ b,
-                                           char* __restrict__ a_next, char* __restrict__ b_next, Rsrc ar, Rsrc br,
-                                           const uint32_t (&a_off)[Tile<kPass, kCols>::kFetchA],
-                                           const uint32_t (&b_off)[Tile<kPass, kCols>::kFetchB], uint32_t ak,
-                                           uint32_t bk, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
-                                           const uint32_t (&b_pos)[2],
-                                           f32x4 (&acc)[Tile<kPass, kCols>::kRT][Tile<kPass, kCols>::kCT]) {
-  typedef Tile<kPass, kCols> T;
-  loss_fetch<T::kFetchA>(ar, a_next, a_off, ak);
-  loss_fetch<T::kFetchB>(br, b_next, b_off, bk);
+// Waits until at most kAhead memory instructions of this wave are under way
+// (kAheadStores if `stored`) and for every wave. The choice is in the assembly:
+// a branch around it would have the compiler keep two copies of the stage, with
+// the sums in other registers.
+template <int kAhead, int kAheadStores>
+__device__ __forceinline__ void landed(int stored) {
+  asm volatile(
+      "s_cmp_lg_u32 %0, 0\n\t"
+      "s_cbranch_scc1 .Lstored%=\n\t"
+      "s_waitcnt vmcnt(%1)\n\t"
+      ".Lstored%=:\n\t"
+      "s_waitcnt vmcnt(%2) lgkmcnt(0)\n\t"
+      "s_barrier" ::"s"(stored),
+      "n"(kAhead), "n"(kAheadStores)
+      : "memory", "scc");
+}
+
+// Nothing moves across: an epilogue handles one 16-column tile after another (the
+// scheduler would read many of them into registers that the products hold).
+__device__ __forceinline__ void order() {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// acc += x y, the sums in the accumulation registers and in place: with the
+// builtin the compiler moves the 256 of them about between stages. A tile's sums
+// are read no sooner than sums_ready() after the last of these (the compiler
+// does not count the matrix core's passes through assembly).
+__device__ __forceinline__ void add_products(f32x4& acc, const bf16x8& x, const bf16x8& y) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
+#endif
+}
+__device__ __forceinline__ void sums_ready() {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// Where a lane reads an operand's half s, and the transposed tiles' swizzle.
+struct ReadPos {
+  uint32_t half[2], turn;
+};
+
+// What the order below leaves to the compiler: address arithmetic, which fits
+// into the products' shadow.
+[[maybe_unused]] constexpr int kOrder = 0x6;  // (vector and scalar ALU instructions may cross)
+
+// Half a stage: the products of the operands in registers and, in a fixed order
+// between them, the reads of the next half's operands and kNA + kNB fetches. Left
+// to the compiler, the fetches go out in one run that the matrix core waits for.
+// The columns' operands come first (all of them are needed for the next half's
+// first products), a row tile's as soon as its products are out, into its place.
+template <Pass kPass, int kCols, int kNA, int kNB, typename Rsrc>
+__device__ __forceinline__ void loss_half(const char* __restrict__ a, const char* __restrict__ b, int s,
+                                          const ReadPos& a_pos, const ReadPos& b_pos, char* __restrict__ a_next,
+                                          char* __restrict__ b_next, Rsrc ar, Rsrc br, const uint32_t (&a_off)[8],
+                                          const uint32_t (&b_off)[Tile<kPass, kCols>::kFetchB], uint32_t ak, uint32_t bk,
+                                          bf16x8 (&x)[8], const bf16x8 (&y)[kCols / 32], bf16x8 (&y_next)[kCols / 32],
+                                          f32x4 (&acc)[8][kCols / 32]) {
+  constexpr int kCT = kCols / 32, kSlots = 4 * kCT;
 #pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    bf16x8 x[T::kRT], y[T::kCT];
+  for (int t = 0; t <= kSlots; ++t) {
+#ifdef __HIP_DEVICE_COMPILE__
+    typedef Tile<kPass, kCols> T;
+    // (B of a wide tile is needed a whole stage later: its fetches go out early)
+    constexpr int kN = kNA + kNB, kSpread = kN && !kNA ? kSlots / 2 : kSlots;
 #pragma unroll
-    for (int i = 0; i < T::kRT; ++i) x[i] = loss_operand<T::kTrA>(a, a_tile + i, s, a_pos[0], a_pos[1]);
+    for (int i = 0; i < kCT; ++i)
+      if (t == 3 * i) y_next[i] = loss_operand<T::kTrB>(b, i, s, b_pos.half[s], b_pos.turn);
 #pragma unroll
-    for (int i = 0; i < T::kCT; ++i) y[i] = loss_operand<T::kTrB>(b, b_tile + i, s, b_pos[0], b_pos[1]);
+    for (int i = 0; i < 8; ++i)
+      if (t == ((i + 1) * kCT + 1) / 2 + (i < 7 ? 1 : 0)) x[i] = loss_operand<T::kTrA>(a, i, s, a_pos.half[s], a_pos.turn);
 #pragma unroll
-    for (int i = 0; i < T::kRT; ++i) {
-#pragma unroll
-      for (int c = 0; c < T::kCT; ++c)
-        acc[i][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[c], acc[i][c], 0, 0, 0);
+    for (int i = 0; i < kN; ++i) {
+      if (t != i * kSpread / (kN ? kN : 1)) continue;
+      if (i < kNA) __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (LdsPtr)(a_next + 1024 * i), 16, a_off[i], ak, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (LdsPtr)(b_next + 1024 * (i - kNA)), 16, b_off[i - kNA], bk, 0, 0);
     }
+    __builtin_amdgcn_sched_barrier(kOrder);
+#endif
+    if (t == kSlots) break;
+#pragma unroll
+    for (int h = 2 * t; h < 2 * t + 2; ++h)
+      add_products(acc[h / kCT][h % kCT], x[h / kCT], y[h % kCT]);
+#ifdef __HIP_DEVICE_COMPILE__
+    __builtin_amdgcn_sched_barrier(kOrder);
+#endif
   }
 }
 
-// Half a stage of the wide tile: 64 products of the operands in registers and,
-// in a fixed order between them, the reads of the next half's operands from `a`
-// and `b` (the columns' first: every product of the next half's first eighth
-// needs them) and the fetches of one operand's tile of a later stage (kSlots of
-// the 16 places for them). Left to the compiler, the fetches go out in one run
-// that the matrix core waits for (dH's product at M 4096, D 2048, 32768
-// vocabulary rows took 490 us).
-template <Pass kPass, int kSlots, typename Rsrc>
-__device__ __forceinline__ void loss_half(const char* __restrict__ a, const char* __restrict__ b,
-                                          char* __restrict__ next, Rsrc rsrc, const uint32_t (&off)[8], uint32_t k,
-                                          int s, int a_tile, int b_tile, const uint32_t (&a_pos)[2],
-                                          const uint32_t (&b_pos)[2], const bf16x8 (&x)[8], const bf16x8 (&y)[8],
-                                          bf16x8 (&x_next)[8], bf16x8 (&y_next)[8], f32x4 (&acc)[8][8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
+// Rows 4 g .. + 3 of tiles a (first) and a + 1 in two words each, exchanged
+// between neighbouring lane groups: 8 rows of tile a + (g & 1) in one lane.
+__device__ __forceinline__ MxU32x4 eight_rows(MxU32x2 first, MxU32x2 second) {
 #ifdef __HIP_DEVICE_COMPILE__
-      typedef Tile<kPass, 256> T;
-      if (h < 2) {
-        const int t = 2 * (i & 3) + h;
-        if (i < 4) y_next[t] = loss_operand<T::kTrB>(b, b_tile + t, s, b_pos[0], b_pos[1]);
-        else x_next[t] = loss_operand<T::kTrA>(a, a_tile + t, s, a_pos[0], a_pos[1]);
-      } else {
-        const int slot = 2 * i + h - 2, n = slot * 8 / kSlots;
-        if (n < 8 && slot * 8 % kSlots == 0)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsPtr)(next + 1024 * n), 16, off[n], k, 0, 0);
-      }
-      __builtin_amdgcn_sched_barrier(0);
+  const auto x = __builtin_amdgcn_permlane16_swap(first.x, second.x, false, false);
+  const auto y = __builtin_amdgcn_permlane16_swap(first.y, second.y, false, false);
+  return MxU32x4{x[0], y[0], x[1], y[1]};
+#else
+  return MxU32x4{first.x, first.y, second.x, second.y};
 #endif
-      acc[i][2 * h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[2 * h], acc[i][2 * h], 0, 0, 0);
-      acc[i][2 * h + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[i], y[2 * h + 1], acc[i][2 * h + 1], 0, 0, 0);
+}
+
+// This wave's 64 of a tile's columns (16 bytes each) into LDS, one wave
+// instruction; columns past M read zeros.
+__device__ __forceinline__ void loss_columns(const LossArgs& p, int c0, int wave, int lane, char* lds) {
 #ifdef __HIP_DEVICE_COMPILE__
-      __builtin_amdgcn_sched_barrier(0);
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)p.columns, (short)0, p.M * 16, kBufferWord3);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * wave), 16, (uint32_t)((c0 + 64 * wave + lane) * 16), 0, 0, 0);
 #endif
-    }
-  }
 }
 
 // The cap, x -> cap tanh(x / cap). Below 5/8 of the cap tanh q = q (1 + s P(s)),
 // s = q^2, P of degree 4 fitted over that range (relative error 2^-27); past it
 // 1 - 2 / (e^2q + 1). Either is within 2e-7 of the cap.
+__device__ constexpr float kCapP[5] = {-0x1.555532p-2f, 0x1.110726p-3f, -0x1.b83c58p-5f, 0x1.52268ep-6f, -0x1.75e194p-8f};
 __device__ __forceinline__ float cap_series(float s) {
-  float u = -0x1.75e194p-8f;
-  u = __builtin_fmaf(u, s, 0x1.52268ep-6f);
-  u = __builtin_fmaf(u, s, -0x1.b83c58p-5f);
-  u = __builtin_fmaf(u, s, 0x1.110726p-3f);
-  u = __builtin_fmaf(u, s, -0x1.555532p-2f);
+  float u = kCapP[4];
+#pragma unroll
+  for (int i = 3; i >= 0; --i) u = __builtin_fmaf(u, s, kCapP[i]);
   return __builtin_fmaf(u, s, 1.0f);
 }
 __device__ __forceinline__ float cap_far(float q) {
   return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(q * (2.0f * kLog2e)) + 1.0f);
 }
-
-// The smallest and the largest of a lane's values of one column.
-template <int kRT, int kCT>
-__device__ __forceinline__ void column_range(const f32x4 (&acc)[kRT][kCT], int b, float& lo, float& hi) {
-  lo = __builtin_inff();
-  hi = -__builtin_inff();
-#pragma unroll
-  for (int a = 0; a < kRT; ++a) {
-    const f32x4 x = acc[a][b];
-    hi = __builtin_fmaxf(__builtin_fmaxf(hi, x[0]), x[1]);
-    hi = __builtin_fmaxf(__builtin_fmaxf(hi, x[2]), x[3]);
-    lo = __builtin_fminf(__builtin_fminf(lo, x[0]), x[1]);
-    lo = __builtin_fminf(__builtin_fminf(lo, x[2]), x[3]);
-  }
+__device__ __forceinline__ float cap_any(float q) {  // tanh q
+  return __builtin_fabsf(q) < kTanhSmall ? q * cap_series(q * q) : cap_far(q);
 }
+
+// The near part in x itself: cap tanh(x / cap) log2(e) = x u(x^2), the powers of
+// 1 / cap and log2(e) in u's coefficients. `far`: where |x| has to stay below
+// (0, never, for caps whose powers leave binary32's range).
+struct CapSeries {
+  float u[6], far;
+  __device__ __forceinline__ CapSeries(float cap) {
+    const float r = 1.0f / cap, r2 = r * r;
+    float c = kLog2e;
+    u[0] = c;
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      c *= r2;
+      u[i + 1] = kCapP[i] * c;
+    }
+    far = cap >= 0x1p-6f && cap <= 0x1p10f ? kTanhSmall * cap : 0.0f;
+  }
+  __device__ __forceinline__ float operator()(float s) const {
+    float v = u[5];
+#pragma unroll
+    for (int i = 4; i >= 0; --i) v = __builtin_fmaf(v, s, u[i]);
+    return v;
+  }
+};
 
 // A (max, sum of exponentials over it) pair with another's.
 __device__ __forceinline__ void join_sums(float& mx, float& sum, float om, float os) {
@@ -226,372 +274,414 @@ __device__ __forceinline__ void join_sums(float& mx, float& sum, float om, float
 }
 
 template <Pass kPass, int kCols, bool kCap>
-__global__ __launch_bounds__((Tile<kPass, kCols>::kThreads), (Tile<kPass, kCols>::kWide ? 1 : 2)) void loss_kernel(
-    LossArgs p) {
+__global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
   typedef Tile<kPass, kCols> T;
+  constexpr int kCT = T::kCT;
   __shared__ __attribute__((aligned(16))) char lds[T::kLds];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4, wr = wave & 1, wc = wave >> 1;
+  const int M = p.M, D = p.D, V = p.V;
+
   // An XCD (consecutive workgroups go to them in turn) takes a run of adjacent
   // tiles, so its workgroups share their operands' lines in its L2: four row
   // tiles by all column tiles (kStats, kGrad), all row tiles by a run of
   // column tiles (kHidden, kWeight).
   const int total = p.row_tiles * p.col_tiles * p.splits;
-  int id = (int)(blockIdx.x & 7) * (int)(gridDim.x >> 3) + (int)(blockIdx.x >> 3);
-  if (id >= total) return;
-  int rt, ct, split = 0;
-  if (kPass == kStats || kPass == kGrad) {
-    const int group = id / (4 * p.col_tiles) * 4;
-    const int in = p.row_tiles - group < 4 ? p.row_tiles - group : 4;
-    id -= group * p.col_tiles;
-    rt = group + id % in;
-    ct = id / in;
-  } else {
-    rt = id % p.row_tiles;
-    id /= p.row_tiles;
-    ct = id % p.col_tiles;
-    split = id / p.col_tiles;
-  }
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4, wr = wave % T::kWavesR, wc = wave / T::kWavesR;
-  const int M = p.M, D = p.D, V = p.V;
-  const int r0 = rt * kRows, c0 = ct * kCols;
+  const int run = (total + 7) / 8, step = (int)(gridDim.x >> 3);
+  int id = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+  const int id_end = ((int)(blockIdx.x & 7) + 1) * run < total ? ((int)(blockIdx.x & 7) + 1) * run : total;
+  if (id >= id_end) return;
+  struct Place {
+    int r0, c0, split;
+  };
+  auto locate = [&](int id) __attribute__((always_inline)) {
+    int rt, ct, split = 0;
+    if (kPass == kStats || kPass == kGrad) {
+      const int group = id / (4 * p.col_tiles) * 4;
+      const int in = p.row_tiles - group < 4 ? p.row_tiles - group : 4;
+      id -= group * p.col_tiles;
+      ct = id / in;
+      rt = group + id - ct * in;
+    } else {
+      const int q = id / p.row_tiles;
+      rt = id - q * p.row_tiles;
+      split = q / p.col_tiles;
+      ct = q - split * p.col_tiles;
+    }
+    return Place{rt * kRows, ct * kCols, split};
+  };
+  auto sums_of_split = [&](int split) __attribute__((always_inline)) {
+    if (kPass != kHidden) return kPass == kWeight ? M : D;
+    const int n = V - split * p.split_rows;
+    return n < 0 ? 0 : n < p.split_rows ? n : p.split_rows;  // (0: a share past the piece's last row, zeros)
+  };
+  auto stages_of = [&](int sums) __attribute__((always_inline)) { return sums > kBlock ? (sums + kBlock - 1) / kBlock : 1; };
 
-  // kGrad: what the epilogue needs of column tid, read now and kept
-  Column column{-1, 0.0f, 0.0f};
-  if (kPass == kGrad && tid < kCols && c0 + tid < M) {
-    const int t = p.targets[c0 + tid];
-    const float most = *p.most;
-    column.target = t < p.vocab ? t : -1;
-    column.ll = -p.lse[c0 + tid] * kLog2e;
-    column.share = most > 0.0f ? p.dloss[c0 + tid] / most : most;
-  }
-
-  // operands: where their first row lies, how many rows there are, their stride
-  const int sum0 = kPass == kHidden ? split * p.split_rows : 0;  // first of the summed index
-  int sums = kPass == kHidden ? (V - sum0 < p.split_rows ? V - sum0 : p.split_rows) : kPass == kWeight ? M : D;
-  if (sums < 0) sums = 0;  // a share past the piece's last row: zeros
-  const uint16_t *A, *B;
-  int a_stride, b_stride, a_bytes, b_bytes;
-  if (kPass == kStats || kPass == kGrad) {
-    const int ra = V - r0 < kRows ? V - r0 : kRows, rb = M - c0 < kCols ? M - c0 : kCols;
-    A = p.W + (size_t)r0 * D;
-    B = p.H + (size_t)c0 * D;
-    a_stride = b_stride = D;
-    a_bytes = ra * D * 2;
-    b_bytes = rb * D * 2;
-  } else if (kPass == kHidden) {
-    const int rb = M - c0 < kCols ? M - c0 : kCols;
-    A = p.W + (size_t)sum0 * D + r0;
-    a_stride = D;
-    a_bytes = (sums * D - r0) * 2;
-    B = p.G + (size_t)c0 * p.g_stride + sum0;
-    b_stride = p.g_stride;
-    b_bytes = (rb * p.g_stride - sum0) * 2;
-    if (sums == 0) a_bytes = b_bytes = 0;
-  } else {
-    A = p.H + r0;
-    a_stride = D;
-    a_bytes = (M * D - r0) * 2;
-    B = p.G + c0;
-    b_stride = p.g_stride;
-    b_bytes = (M * p.g_stride - c0) * 2;
-  }
-  const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc((void*)A, (short)0, a_bytes, kBufferWord3);
-  const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void*)B, (short)0, b_bytes, kBufferWord3);
-
-  // fetch offsets and read positions. Rows of 64 (128 bytes): 16-byte chunk c of
-  // row r lands at chunk c ^ (r & 7). Transposed tiles: rows of 256 (512 bytes).
-  uint32_t a_off[T::kFetchA], b_off[T::kFetchB], a_pos[2], b_pos[2];
-  const uint32_t nat0 = (uint32_t)(j * 128 + ((g ^ (j & 7)) * 16)), nat1 = (uint32_t)(j * 128 + (((4 + g) ^ (j & 7)) * 16));
-  const uint32_t tr0 = (uint32_t)((8 * g + (j >> 2)) * 512 + (j & 3) * 8), tr1 = (uint32_t)(((j >> 2) | ((g & 1) << 2)) * 32);
-  // row of this lane in fetch i of a transposed tile (the same for both operands, where both are)
-  auto turned_row = [&](int i) __attribute__((always_inline)) { return 64 / T::kWaves * wave + 2 * i + (lane >> 5); };
+  // ---- fetches: where this lane's 16 bytes of each wave instruction come from
+  const int a_stride = D, b_stride = kPass == kStats || kPass == kGrad ? D : p.g_stride;
+  const uint32_t a_step = T::kTrA ? (uint32_t)(kBlock * a_stride * 2) : kBlock * 2;
+  const uint32_t b_step = T::kTrB ? (uint32_t)(kBlock * b_stride * 2) : kBlock * 2;
+  // Rows of 64 (128 bytes): 16-byte chunk c of row r lands at chunk c ^ (r & 7).
+  // Transposed tiles: rows of 256 (512 bytes), pairs of chunks swizzled.
+  auto turned_row = [&](int i) __attribute__((always_inline)) { return 16 * wave + 2 * i + (lane >> 5); };
+  auto turned_chunk = [&](int i) __attribute__((always_inline)) {
+    return (((lane & 31) >> 1) ^ pair_swizzle(turned_row(i))) * 2 + (lane & 1);
+  };
   auto natural = [&](int row, int stride) __attribute__((always_inline)) {
     return (uint32_t)(row * stride * 2 + ((lane & 7) ^ (lane >> 3)) * 16);
   };
-  auto turned = [&](int i, int stride, int cols) __attribute__((always_inline)) {
-    const int row = turned_row(i), c = (((lane & 31) >> 1) ^ pair_swizzle(row)) * 2 + (lane & 1);
-    return 8 * c < cols ? (uint32_t)(row * stride * 2 + c * 16) : kBufferOutOfRange;
-  };
+  uint32_t a_off[8], b_off[T::kFetchB];
 #pragma unroll
-  for (int i = 0; i < T::kFetchA; ++i)
-    a_off[i] = T::kTrA ? turned(i, a_stride, D - r0) : natural(kRows / T::kWaves * wave + 8 * i + (lane >> 3), a_stride);
+  for (int i = 0; i < 8; ++i) a_off[i] = T::kTrA ? 0u : natural(64 * wave + 8 * i + (lane >> 3), a_stride);
 #pragma unroll
   for (int i = 0; i < T::kFetchB; ++i)
-    b_off[i] = T::kTrB ? turned(i, b_stride, 256) : natural(kCols / T::kWaves * wave + 8 * i + (lane >> 3), b_stride);
-  a_pos[0] = T::kTrA ? tr0 : nat0;
-  a_pos[1] = T::kTrA ? tr1 : nat1;
-  b_pos[0] = T::kTrB ? tr0 : nat0;
-  b_pos[1] = T::kTrB ? tr1 : nat1;
-
-  f32x4 acc[T::kRT][T::kCT];
-#pragma unroll
-  for (int a = 0; a < T::kRT; ++a) {
-#pragma unroll
-    for (int b = 0; b < T::kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-  const int nk = (sums + kBlock - 1) / kBlock;
+    b_off[i] = T::kTrB ? (uint32_t)(turned_row(i) * b_stride * 2 + turned_chunk(i) * 16)
+                       : natural(kCols / 4 * wave + 8 * i + (lane >> 3), b_stride);
   // W's rows are read at other columns on other XCDs, which spreads them over the memory channels
-  const int first = kPass == kStats || kPass == kGrad ? (int)(blockIdx.x & 7) * nk / 8 : 0;
-  auto at = [&](int kb) __attribute__((always_inline)) {
-    const int k = (kb < nk ? kb : 0) + first;  // (within the operands also where nothing is fetched)
-    return (uint32_t)(k < nk ? k : k - nk);
-  };
-  const uint32_t a_step = T::kTrA ? (uint32_t)(kBlock * a_stride * 2) : kBlock * 2;
-  const uint32_t b_step = T::kTrB ? (uint32_t)(kBlock * b_stride * 2) : kBlock * 2;
-  // A stage past the last is fetched as nothing (zeros); in the last stage of a
-  // sum over rows, rows past it are too.
-  auto offsets_a = [&](int kb, uint32_t (&ao)[T::kFetchA]) __attribute__((always_inline)) {
-    const uint32_t none = kb < nk ? 0u : kBufferOutOfRange;
-    const int rows = sums - (int)at(kb) * kBlock;
-#pragma unroll
-    for (int i = 0; i < T::kFetchA; ++i) ao[i] = a_off[i] | (T::kTrA && turned_row(i) >= rows ? kBufferOutOfRange : none);
-  };
-  auto offsets_b = [&](int kb, uint32_t (&bo)[T::kFetchB]) __attribute__((always_inline)) {
-    const uint32_t none = kb < nk ? 0u : kBufferOutOfRange;
-    const int rows = sums - (int)at(kb) * kBlock;
-#pragma unroll
-    for (int i = 0; i < T::kFetchB; ++i) bo[i] = b_off[i] | (T::kTrB && turned_row(i) >= rows ? kBufferOutOfRange : none);
-  };
-  const int a_dst = T::kA / T::kWaves * wave, b_dst = T::kB / T::kWaves * wave;
-  const int a_tile = T::kRT * wr, b_tile = T::kCT * wc;
-  auto fetch = [&](int kb, char* a, char* b) __attribute__((always_inline)) {
-    uint32_t ao[T::kFetchA], bo[T::kFetchB];
-    offsets_a(kb, ao);
-    offsets_b(kb, bo);
-    loss_fetch<T::kFetchA>(ar, a + a_dst, ao, at(kb) * a_step);
-    loss_fetch<T::kFetchB>(br, b + b_dst, bo, at(kb) * b_step);
-  };
-  if constexpr (T::kWide) {
-    // The stages' tiles (A, B, A, B, ...) take five places in turn. A stage's
-    // operands are in registers half a stage before its last products, so from
-    // the middle of stage k on its two places are free: B of stage k + 2 is
-    // fetched into the one in the second half (early in it), A of stage k + 3
-    // into the other in the next stage's first half, and both have landed by the
-    // middle of the stage before theirs. (All fetches in the second half, into
-    // two whole buffers, took 3% more.)
-    bf16x8 x0[8], y0[8], x1[8], y1[8];
-    fetch(0, lds, lds + T::kA);
-    fetch(1, lds + 2 * T::kA, lds + 3 * T::kA);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFetches) : "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      x0[i] = loss_operand<T::kTrA>(lds, a_tile + i, 0, a_pos[0], a_pos[1]);
-      y0[i] = loss_operand<T::kTrB>(lds + T::kA, b_tile + i, 0, b_pos[0], b_pos[1]);
-    }
-    for (int kb = 0; kb < nk; kb += 5) {
-#pragma unroll
-      for (int u = 0; u < 5; ++u) {
-        if (kb + u < nk) {
-          const char *a = lds + 2 * u % 5 * T::kA, *b = lds + (2 * u + 1) % 5 * T::kA;
-          const char *a1 = lds + (2 * u + 2) % 5 * T::kA, *b1 = lds + (2 * u + 3) % 5 * T::kA;
-          char *a2 = lds + (2 * u + 4) % 5 * T::kA, *b2 = lds + 2 * u % 5 * T::kA;
-          const int n = kb + u + 2;
-          uint32_t off[8];
-          offsets_a(n, off);
-          loss_half<kPass, 16>(a, b, a2 + a_dst, ar, off, at(n) * a_step, 1, a_tile, b_tile, a_pos, b_pos, x0, y0, x1,
-                               y1, acc);
-          // the next stage has landed for every wave, and every wave has read this one
-          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(T::kFetchA) : "memory");
-          offsets_b(n, off);
-          loss_half<kPass, 8>(a1, b1, b2 + b_dst, br, off, at(n) * b_step, 0, a_tile, b_tile, a_pos, b_pos, x1, y1, x0,
-                              y0, acc);
+  const int first = kPass == kStats || kPass == kGrad ? (int)(blockIdx.x & 7) * (D / kBlock) / 8 : 0;
+  // the tile and the stage that are fetched next
+  __amdgpu_buffer_rsrc_t ar, br;
+  int f_id = id, f_left = 0, f_nk = 0, f_k = 0, f_sums = 0;
+  uint32_t f_ak = 0, f_bk = 0;
+  // (The resources end with the last summed row, and the offset of a stage counts
+  // in their bounds check: rows past it are read as zeros.)
+  auto fetch_tile = [&]() __attribute__((always_inline)) {
+    int t = f_id;
+    asm volatile("" : "+s"(t));  // (nothing of this is computed ahead of the branch here)
+    const uint16_t *A = p.W, *B = p.H;
+    int a_bytes = 0, b_bytes = 0;  // past the last tile: nothing is read
+    f_sums = 0;
+    f_nk = f_left = 1;
+    f_k = 0;
+    if (t < id_end) {
+      const Place q = locate(t);
+      f_sums = sums_of_split(q.split);
+      f_nk = f_left = stages_of(f_sums);
+      f_k = first;
+      if (kPass == kStats || kPass == kGrad) {
+        A = p.W + (size_t)q.r0 * D;
+        B = p.H + (size_t)q.c0 * D;
+        a_bytes = (V - q.r0 < kRows ? V - q.r0 : kRows) * D * 2;
+        b_bytes = (M - q.c0 < kCols ? M - q.c0 : kCols) * D * 2;
+      } else if (f_sums > 0) {
+        const int sum0 = kPass == kHidden ? q.split * p.split_rows : 0;
+        if (kPass == kHidden) {
+          A = p.W + (size_t)sum0 * D + q.r0;
+          B = p.G + (size_t)q.c0 * p.g_stride + sum0;
+          b_bytes = ((M - q.c0 < kCols ? M - q.c0 : kCols) * p.g_stride - sum0) * 2;
+        } else {
+          A = p.H + q.r0;
+          B = p.G + q.c0;
+          b_bytes = (M * p.g_stride - q.c0) * 2;
         }
+        a_bytes = (f_sums * D - q.r0) * 2;
+      }
+      if (T::kTrA) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          a_off[i] = 8 * turned_chunk(i) < D - q.r0 ? (uint32_t)(turned_row(i) * a_stride * 2 + turned_chunk(i) * 16)
+                                                    : kBufferOutOfRange;
       }
     }
-  } else {
-#pragma unroll
-    for (int u = 0; u < T::kStages - 1; ++u) fetch(u, lds + u * T::kStage, lds + u * T::kStage + T::kA);
-    for (int kb = 0; kb < nk; kb += T::kStages) {
-#pragma unroll
-      for (int u = 0; u < T::kStages; ++u) {
-        if (kb + u < nk) {
-          // the stage has landed for every wave, and every wave has read the one before
-          asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
-          const int n = kb + u + T::kStages - 1;
-          char* next = lds + (u + T::kStages - 1) % T::kStages * T::kStage;
-          const char* cur = lds + u * T::kStage;
-          uint32_t ao[T::kFetchA], bo[T::kFetchB];
-          offsets_a(n, ao);
-          offsets_b(n, bo);
-          loss_block<kPass, kCols>(cur, cur + T::kA, next + a_dst, next + T::kA + b_dst, ar, br, ao, bo, at(n) * a_step,
-                                   at(n) * b_step, a_tile, b_tile, a_pos, b_pos, acc);
-        }
-      }
+    ar = __builtin_amdgcn_make_buffer_rsrc((void*)A, (short)0, a_bytes, kBufferWord3);
+    br = __builtin_amdgcn_make_buffer_rsrc((void*)B, (short)0, b_bytes, kBufferWord3);
+    f_ak = (uint32_t)f_k * a_step;
+    f_bk = (uint32_t)f_k * b_step;
+  };
+  auto fetch_next = [&]() __attribute__((always_inline)) {
+    if (--f_left == 0) {
+      f_id = f_id < id_end ? f_id + step : f_id;
+      fetch_tile();
+    } else {
+      const bool wrap = ++f_k == f_nk;
+      f_k = wrap ? 0 : f_k;
+      f_ak = wrap ? 0u : f_ak + a_step;
+      f_bk = wrap ? 0u : f_bk + b_step;
     }
-  }
-  // nothing is in flight to or from LDS before the epilogue uses it
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  const int a_dst = T::kA / 4 * wave, b_dst = T::kB / 4 * wave;
 
-  if constexpr (kPass == kGrad) {
-    // the columns' values behind the staged outputs
-    if (tid < kCols) ((Column*)(lds + T::kOut))[tid] = column;
-    __syncthreads();
+  // ---- reads: lane (j, g) holds the summed index 8 g .. + 7 of a half for row (column) j of a tile
+  ReadPos a_pos, b_pos;
+  {
+    const uint32_t nat0 = (uint32_t)(j * 128 + ((g ^ (j & 7)) * 16)), nat1 = (uint32_t)(j * 128 + (((4 + g) ^ (j & 7)) * 16));
+    const uint32_t tr = (uint32_t)((8 * g + (j >> 2)) * 512 + (j & 3) * 8), turn = (uint32_t)(((j >> 2) | ((g & 1) << 2)) * 32);
+    a_pos.half[0] = T::kTrA ? tr + 256 * wr : nat0 + 16384 * wr;  // (a wave's tiles start at a multiple of 8)
+    a_pos.half[1] = T::kTrA ? tr + 256 * wr : nat1 + 16384 * wr;
+    a_pos.turn = turn;
+    b_pos.half[0] = T::kTrB ? tr + 256 * wc : nat0 + 2048 * kCT * wc;
+    b_pos.half[1] = T::kTrB ? tr + 256 * wc : nat1 + 2048 * kCT * wc;
+    b_pos.turn = turn;
   }
-  // lane (j, g) holds rows 16 a + 4 g + e and column 16 b + j of its wave's tile
-  const int row0 = 16 * T::kRT * wr + 4 * g, col0 = 16 * T::kCT * wc + j;
-  if constexpr (kPass == kStats) {
-    const float rcap = kCap ? 1.0f / p.cap : 0.0f, rcap2 = rcap * rcap, far = kTanhSmall * p.cap;
-    const bool tail = V - r0 < kRows;  // (uniform) rows past the vocabulary count nothing
-    float2* sums_of = (float2*)lds;    // [kWavesR][kCols]
+
+  // ---- the first stages
+  fetch_tile();
 #pragma unroll
-    for (int b = 0; b < T::kCT; ++b) {
-      if (tail) {
+  for (int u = 0; u < (T::kFive ? 2 : 3); ++u) {
+    [[maybe_unused]] char* a = lds + (T::kFive ? 2 * u * T::kA : u * T::kPlace);
+#ifdef __HIP_DEVICE_COMPILE__
 #pragma unroll
-        for (int a = 0; a < T::kRT; ++a) {
+    for (int i = 0; i < 8; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ar, (LdsPtr)(a + a_dst + 1024 * i), 16, a_off[i], f_ak, 0, 0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (r0 + row0 + 16 * a + e >= V) acc[a][b][e] = -__builtin_inff();
-        }
-      }
-      float lo, mx, sum = 0.0f;
-      column_range(acc, b, lo, mx);
-      if (!kCap) {
-        mx = __builtin_fmaxf(mx, kLowest);
-        const float ml = -mx * kLog2e;
+    for (int i = 0; i < T::kFetchB; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(br, (LdsPtr)(a + T::kA + b_dst + 1024 * i), 16, b_off[i], f_bk, 0, 0);
+#endif
+    fetch_next();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((T::kFive ? 1 : 2) * (8 + T::kFetchB)) : "memory");
+
+  // ---- tile after tile
+  // the ring: where a stage's operands and the next ones lie (bytes into lds)
+  int ring[T::kFive ? 5 : 3];
 #pragma unroll
-        for (int a = 0; a < T::kRT; ++a) {
+  for (int i = 0; i < (T::kFive ? 5 : 3); ++i) ring[i] = i * T::kPlace;
+  int stored = 0;  // a tile has just been stored
+  for (; id < id_end; id += step) {
+    f32x4 acc[8][kCT];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, ml));
-        }
+    for (int a = 0; a < 8; ++a) {
+#pragma unroll
+      for (int b = 0; b < kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    bf16x8 x[8], y0[kCT], y1[kCT];
+    {
+      const char *a = lds + ring[0], *b = lds + (T::kFive ? ring[1] : ring[0] + T::kA);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = loss_operand<T::kTrA>(a, i, 0, a_pos.half[0], a_pos.turn);
+#pragma unroll
+      for (int i = 0; i < kCT; ++i) y0[i] = loss_operand<T::kTrB>(b, i, 0, b_pos.half[0], b_pos.turn);
+    }
+    const Place here = locate(id);
+    const int nk = stages_of(sums_of_split(here.split));
+    char* scratch = lds + T::kOperands;
+    for (int kb = 0; kb < nk; ++kb) {
+      const bool last = kb + 1 == nk;
+      if constexpr (T::kFive) {
+        // places: this stage's A and B, the next one's, and a free one, which takes
+        // A of the stage after; its B takes this A's place from the middle on
+        char *a = lds + ring[0], *b = lds + ring[1], *a1 = lds + ring[2], *b1 = lds + ring[3], *a2 = lds + ring[4];
+        scratch = b;  // read by the middle of the stage, and not yet taken again
+        loss_half<kPass, kCols, 8, 0>(a, b, 1, a_pos, b_pos, a2 + a_dst, nullptr, ar, br, a_off, b_off, f_ak, f_bk, x, y0, y1, acc);
+        // the next stage has landed for every wave, and every wave has read this one
+        landed<T::kAhead, T::kAheadStores>(stored);
+        if (kPass == kGrad && last) loss_columns(p, here.c0, wave, lane, scratch);
+        loss_half<kPass, kCols, 0, T::kFetchB>(a1, b1, 0, a_pos, b_pos, nullptr, a + b_dst, ar, br, a_off, b_off, f_ak, f_bk,
+                                               x, y1, y0, acc);
+        const int r0 = ring[0], r1 = ring[1];
+        ring[0] = ring[2];
+        ring[1] = ring[3];
+        ring[2] = ring[4];
+        ring[3] = r0;
+        ring[4] = r1;
       } else {
-        const bool near = lo > -far && mx < far;  // (false with a NaN about, or a masked row)
-        mx = p.cap * cap_far(mx * rcap);          // tanh keeps the order
-        const float ml = -mx * kLog2e;
-        if (__all(near)) {
+        char *cur = lds + ring[0], *next = lds + ring[1];
+        loss_half<kPass, kCols, 0, 0>(cur, cur + T::kA, 1, a_pos, b_pos, nullptr, nullptr, ar, br, a_off, b_off, 0, 0, x, y0,
+                                      y1, acc);
+        landed<T::kAhead, T::kAheadStores>(stored);
+        if (kPass == kGrad && last) loss_columns(p, here.c0, wave, lane, scratch);
+        loss_half<kPass, kCols, 8, T::kFetchB>(next, next + T::kA, 0, a_pos, b_pos, cur + a_dst, cur + T::kA + b_dst, ar, br,
+                                               a_off, b_off, f_ak, f_bk, x, y1, y0, acc);
+        const int r0 = ring[0];
+        ring[0] = ring[1];
+        ring[1] = ring[2];
+        ring[2] = r0;
+      }
+      fetch_next();
+      asm volatile("s_mov_b32 %0, 0" : "=s"(stored));  // (a constant from here on would have the first stage peeled)
+    }
+
+    sums_ready();
+    // ---- the tile is done: lane (j, g) holds rows 16 a + 4 g + e and column 16 b + j of its wave's part
+    const int r0 = here.r0, c0 = here.c0;
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (what follows is computed here, not kept in registers over the products)
+    const int ej = l & 15, eg = l >> 4;
+    const int row0 = 128 * wr + 4 * eg, col0 = 16 * kCT * wc + ej;
+    const int row8 = 128 * wr + 16 * (eg & 1) + 4 * (eg & 2);  // after an exchange: 8 rows from 16 a + this on, a even
+    const bool tail = V - r0 < kRows;  // (uniform; kStats, kGrad) the tile ends past the vocabulary
+    if constexpr (kPass == kStats) {
+      const CapSeries series(p.cap);
+      float2* sums_of = (float2*)scratch;  // [2][kCols]
 #pragma unroll
-          for (int a = 0; a < T::kRT; ++a) {
+      for (int b = 0; b < kCT; ++b) {
+        order();
+        if (tail) {  // rows past the vocabulary count nothing
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = acc[a][b][e], s = x * (x * rcap2);
-              sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x * kLog2e, cap_series(s), ml));
-            }
+          for (int a = 0; a < 8; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r0 + row0 + 16 * a + e >= V) acc[a][b][e] = -__builtin_inff();
+          }
+        }
+        float lo = __builtin_inff(), mx = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+          const f32x4 x = acc[a][b];
+          mx = __builtin_fmaxf(__builtin_fmaxf(mx, x[0]), x[1]);
+          mx = __builtin_fmaxf(__builtin_fmaxf(mx, x[2]), x[3]);
+          if (kCap) {
+            lo = __builtin_fminf(__builtin_fminf(lo, x[0]), x[1]);
+            lo = __builtin_fminf(__builtin_fminf(lo, x[2]), x[3]);
+          }
+        }
+        if (!kCap) {
+          mx = __builtin_fmaxf(mx, kLowest);
+          const float ml = -mx * kLog2e;
+#pragma unroll
+          for (int a = 0; a < 8; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, ml));
           }
         } else {
+          const bool near = lo > -series.far && mx < series.far;  // (false with a masked row; a NaN stays one either way)
+          mx = p.cap * cap_far(mx / p.cap);                       // tanh keeps the order
+          const float ml = -mx * kLog2e;
+          if (__all(near)) {
 #pragma unroll
-          for (int a = 0; a < T::kRT; ++a) {
+            for (int a = 0; a < 8; ++a) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = acc[a][b][e], q = x * rcap;
-              const float z = __builtin_fabsf(q) < kTanhSmall ? x * cap_series(q * q) : p.cap * cap_far(q);
-              const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(z, kLog2e, ml));
-              sum += tail && r0 + row0 + 16 * a + e >= V ? 0.0f : v;
+              for (int e = 0; e < 4; ++e) {
+                const float x = acc[a][b][e];
+                sum += __builtin_amdgcn_exp2f(__builtin_fmaf(x, series(x * x), ml));
+              }
+            }
+          } else {
+#pragma unroll
+            for (int a = 0; a < 8; ++a) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(p.cap * cap_any(acc[a][b][e] / p.cap), kLog2e, ml));
+                sum += tail && r0 + row0 + 16 * a + e >= V ? 0.0f : v;
+              }
             }
           }
         }
+        // the four lane groups of a column
+#pragma unroll
+        for (int d = 16; d < 64; d <<= 1) join_sums(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
+        if (eg == 0) sums_of[wr * kCols + col0 + 16 * b] = make_float2(mx, sum);
       }
-      // the four lane groups of a column
-#pragma unroll
-      for (int d = 16; d < 64; d <<= 1) join_sums(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
-      if (g == 0) sums_of[wr * kCols + col0 + 16 * b] = make_float2(mx, sum);
-    }
-    __syncthreads();
-    if (tid < kCols && c0 + tid < M) {
-      float2 s = sums_of[tid];
-#pragma unroll
-      for (int w = 1; w < T::kWavesR; ++w) {
-        const float2 o = sums_of[w * kCols + tid];
+      lds_barrier();
+      if (tid < kCols && c0 + tid < M) {
+        float2 s = sums_of[tid];
+        const float2 o = sums_of[kCols + tid];
         join_sums(s.x, s.y, o.x, o.y);
+        p.stats[(size_t)(r0 / kRows) * M + c0 + tid] = s;
       }
-      p.stats[(size_t)rt * M + c0 + tid] = s;
-    }
-  } else if constexpr (kPass == kGrad) {
-    const float rcap = kCap ? 1.0f / p.cap : 0.0f, rcap2 = rcap * rcap, far = kTanhSmall * p.cap;
-    uint16_t* stage = (uint16_t*)lds;
+      lds_barrier();  // read before a fetch takes the place
+    } else if constexpr (kPass == kGrad) {
+      const CapSeries series(p.cap);
+      const float per_cap2 = 1.0f / (p.cap * kLog2e) / (p.cap * kLog2e);
+      // the columns' values have landed for every wave; the next tile's fetches may be under way
+      asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFive ? T::kFetchB : 8 + T::kFetchB) : "memory");
+      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.G + (size_t)c0 * p.g_stride), (short)0, (M - c0 < kCols ? M - c0 : kCols) * p.g_stride * 2, kBufferWord3);
 #pragma unroll
-    for (int b = 0; b < T::kCT; ++b) {
-      const int col = col0 + 16 * b;
-      const Column c = ((const Column*)(lds + T::kOut))[col];
-      const bool scored = c.target >= 0;
-      const float ll = c.ll, share = c.share;
-      const int hit = c.target - p.v_base - r0 - row0;  // the target's place among this lane's rows
-      const bool any_hit = __any(scored && hit >= 0 && hit < 16 * T::kRT);
-      bool near = true;
-      if (kCap) {
-        float lo, hi;
-        column_range(acc, b, lo, hi);
-        near = __all(lo > -far && hi < far);
-      }
+      for (int b = 0; b < kCT; ++b) {
+        order();
+        const int col = col0 + 16 * b;
+        const Column c = ((const Column*)scratch)[col];
+        const bool scored = c.target >= 0;
+        const int hit = c.target - p.v_base - r0 - row0;  // the target's place among this lane's rows
+        const bool any_hit = __any(scored && hit >= 0 && hit < 128);
+        bool near = true;
+        if (kCap) {
+          float most = 0.0f;
 #pragma unroll
-      for (int a = 0; a < T::kRT; ++a) {
-        float v[4], w[4];
+          for (int a = 0; a < 8; ++a) {
+            const f32x4 x = acc[a][b];
+            most = __builtin_fmaxf(__builtin_fmaxf(most, __builtin_fabsf(x[0])), __builtin_fabsf(x[1]));
+            most = __builtin_fmaxf(__builtin_fmaxf(most, __builtin_fabsf(x[2])), __builtin_fabsf(x[3]));
+          }
+          near = __all(most < series.far);
+        }
+        if (kCap && !near) {  // (uniform) z in x's place
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float x = acc[a][b][e];
-          w[e] = 1.0f;
-          if (!kCap) {
-            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, ll));
-          } else if (near) {
-            const float s = x * (x * rcap2), u = cap_series(s);
-            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x * kLog2e, u, ll));
-            w[e] = __builtin_fmaf(-s, u * u, 1.0f);
-          } else {
-            const float q = x * rcap;
-            const float t = __builtin_fabsf(q) < kTanhSmall ? q * cap_series(q * q) : cap_far(q);
-            v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p.cap * t, kLog2e, ll));
-            w[e] = __builtin_fmaf(-t, t, 1.0f);
+          for (int a = 0; a < 8; ++a) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[a][b][e] = p.cap * kLog2e * cap_any(acc[a][b][e] / p.cap);
           }
         }
-        if (any_hit) {  // (uniform)
+        MxU32x2 w[8];
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hit == 16 * a + e) v[e] -= 1.0f;
+        for (int a = 0; a < 8; ++a) {
+          float v[4], slope[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = acc[a][b][e];
+            if (!kCap) {
+              v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, c.ll));
+              slope[e] = c.share;
+            } else {
+              // z log2(e), and share (1 - (z / cap)^2)
+              const float z = near ? x * series(x * x) : x;
+              v[e] = __builtin_amdgcn_exp2f(z + c.ll);
+              slope[e] = __builtin_fmaf(z * z, -per_cap2 * c.share, c.share);
+            }
+          }
+          if (any_hit) {  // (uniform)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (hit == 16 * a + e) v[e] -= 1.0f;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] *= slope[e];
+          if (tail) {  // zeros past the vocabulary
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (r0 + row0 + 16 * a + e >= V) v[e] = 0.0f;
+          }
+          // a row that is not scored has no gradient, whatever its hidden state holds
+          w[a] = MxU32x2{scored ? pack_bf16(v[0], v[1]) : 0u, scored ? pack_bf16(v[2], v[3]) : 0u};
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= kCap ? w[e] * share : share;
-        if (V - r0 < kRows) {  // (uniform) zeros past the vocabulary
+        for (int a = 0; a < 8; a += 2)
+          __builtin_amdgcn_raw_buffer_store_b128(eight_rows(w[a], w[a + 1]), out,
+                                                 (uint32_t)((col * p.g_stride + r0 + row8 + 16 * a) * 2), 0, 0);
+      }
+      lds_barrier();  // the columns' values are read before a fetch takes the place
+    } else if constexpr (kPass == kHidden) {
+      const int rows = M - c0 < kCols ? M - c0 : kCols;
+      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.part + ((size_t)here.split * M + c0) * D), (short)0, rows * D * 4, kBufferWord3);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (r0 + row0 + 16 * a + e >= V) v[e] = 0.0f;
+      for (int b = 0; b < kCT; ++b) {
+        order();
+        uint32_t o[8];
+        f32x4 v[8];
+#pragma unroll
+        for (int a = 0; a < 8; ++a) {
+          const int k = r0 + row0 + 16 * a;
+          o[a] = k < D ? (uint32_t)(((col0 + 16 * b) * D + k) * 4) : kBufferOutOfRange;
+          v[a] = acc[a][b];
+          if (p.accumulate) v[a] += __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(out, o[a], 0, 0));
         }
-        // a row that is not scored has no gradient, whatever its hidden state holds
-        const MxU32x2 o = {scored ? pack_bf16(v[0], v[1]) : 0u, scored ? pack_bf16(v[2], v[3]) : 0u};
-        *(MxU32x2*)&stage[col * T::kOutStride + row0 + 16 * a] = o;
+#pragma unroll
+        for (int a = 0; a < 8; ++a) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(MxU32x4, v[a]), out, o[a], 0, 0);
       }
-    }
-    __syncthreads();
-    // rows of 512 bytes of g
-#pragma unroll 4
-    for (int q = tid; q < kCols * 32; q += T::kThreads) {
-      const int m = q >> 5, c = (q & 31) * 8;
-      if (c0 + m < M)
-        *(MxU32x4*)&p.G[(size_t)(c0 + m) * p.g_stride + r0 + c] = *(const MxU32x4*)&stage[m * T::kOutStride + c];
-    }
-  } else if constexpr (kPass == kHidden) {
-    float* part = p.part + (size_t)split * M * D;
+    } else {
+      const float most = *p.most;
+      const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
+          (void*)(p.dW + (size_t)c0 * D), (short)0, (V - c0 < kCols ? V - c0 : kCols) * D * 2, kBufferWord3);
 #pragma unroll
-    for (int b = 0; b < T::kCT; ++b) {
-      const int m = c0 + col0 + 16 * b;
+      for (int b = 0; b < kCT; ++b) {
+        order();
 #pragma unroll
-      for (int a = 0; a < T::kRT; ++a) {
-        const int k = r0 + row0 + 16 * a;
-        if (m < M && k < D) {
-          f32x4* o = (f32x4*)&part[(size_t)m * D + k];
-          f32x4 v = acc[a][b];
-          if (p.accumulate) v += *o;
-          *o = v;
+        for (int a = 0; a < 8; a += 2) {
+          const f32x4 v = acc[a][b] * most, u = acc[a + 1][b] * most;
+          const int k = r0 + row8 + 16 * a;
+          __builtin_amdgcn_raw_buffer_store_b128(
+              eight_rows(MxU32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])},
+                         MxU32x2{pack_bf16(u[0], u[1]), pack_bf16(u[2], u[3])}),
+              out, k < D ? (uint32_t)(((col0 + 16 * b) * D + k) * 2) : kBufferOutOfRange, 0, 0);
         }
       }
     }
-  } else {
-    uint16_t* stage = (uint16_t*)lds;
-    const float most = *p.most;
-#pragma unroll
-    for (int b = 0; b < T::kCT; ++b) {
-#pragma unroll
-      for (int a = 0; a < T::kRT; ++a) {
-        const f32x4 v = acc[a][b] * most;
-        *(MxU32x2*)&stage[(col0 + 16 * b) * T::kOutStride + row0 + 16 * a] =
-            MxU32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-      }
-    }
-    __syncthreads();
-#pragma unroll 4
-    for (int q = tid; q < kCols * 32; q += T::kThreads) {
-      const int v = q >> 5, c = (q & 31) * 8;
-      if (c0 + v < V && r0 + c < D)
-        *(MxU32x4*)&p.dW[(size_t)(c0 + v) * D + r0 + c] = *(const MxU32x4*)&stage[v * T::kOutStride + c];
-    }
+    stored = 1;
   }
+  // no fetch is under way to LDS that the next workgroup may get
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // lse and loss of 8 rows a workgroup: the tiles' (max, sum) joined in one
@@ -648,10 +738,11 @@ __global__ __launch_bounds__(256) void loss_join_kernel(const float2* __restrict
 }
 
 // The largest |dloss| of the scored rows (a NaN stays one: its bits are above
-// every number's).
-__global__ __launch_bounds__(1024) void loss_scale_kernel(const float* __restrict__ dloss,
-                                                          const int32_t* __restrict__ targets, int M, int V,
-                                                          float* __restrict__ most) {
+// every number's), and then every row's values for kGrad.
+__global__ __launch_bounds__(1024) void loss_columns_kernel(const float* __restrict__ dloss,
+                                                            const int32_t* __restrict__ targets,
+                                                            const float* __restrict__ lse, int M, int V,
+                                                            float* __restrict__ most, Column* __restrict__ columns) {
   __shared__ uint32_t wave_most[16];
   uint32_t b = 0;
   for (int m = threadIdx.x; m < M; m += 1024) {
@@ -666,9 +757,13 @@ __global__ __launch_bounds__(1024) void loss_scale_kernel(const float* __restric
   }
   if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = b;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 16; ++i) b = wave_most[i] > b ? wave_most[i] : b;
-    *most = __uint_as_float(b);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) b = wave_most[i] > b ? wave_most[i] : b;
+  const float top = __uint_as_float(b);
+  if (threadIdx.x == 0) *most = top;
+  for (int m = threadIdx.x; m < M; m += 1024) {
+    const int t = targets[m];
+    columns[m] = Column{t < V ? t : -1, -lse[m] * kLog2e, top > 0.0f ? dloss[m] / top : top, 0.0f};
   }
 }
 
@@ -708,32 +803,32 @@ __global__ __launch_bounds__(256) void loss_hidden_kernel(const float* __restric
   store_8<true>(dH, e, 8, v);
 }
 
-template <Pass kPass, bool kCap>
-void loss_launch_capped(const LossArgs& p, int cols, hipStream_t s) {
+template <Pass kPass, int kCols>
+void loss_launch_cols(const LossArgs& p, int cus, hipStream_t s) {
   const int total = p.row_tiles * p.col_tiles * p.splits;
-  const dim3 grid((unsigned)((total + 7) / 8 * 8));
-  if constexpr (kPass != kWeight) {
-    if (cols == 64) {
-      loss_kernel<kPass, 64, kCap><<<grid, dim3(Tile<kPass, 64>::kThreads), 0, s>>>(p);
-      return;
-    }
-    if (cols == 128) {
-      loss_kernel<kPass, 128, kCap><<<grid, dim3(Tile<kPass, 128>::kThreads), 0, s>>>(p);
+  const dim3 grid((unsigned)std::min((total + 7) / 8 * 8, std::max(8, cus / 8 * 8))), block(kLossThreads);
+  if constexpr (kPass == kStats || kPass == kGrad) {
+    if (p.cap > 0.0f) {
+      loss_kernel<kPass, kCols, true><<<grid, block, 0, s>>>(p);
       return;
     }
   }
-  loss_kernel<kPass, 256, kCap><<<grid, dim3(Tile<kPass, 256>::kThreads), 0, s>>>(p);
+  loss_kernel<kPass, kCols, false><<<grid, block, 0, s>>>(p);
 }
 
 template <Pass kPass>
-void loss_launch(const LossArgs& p, int cols, hipStream_t s) {
-  if constexpr (kPass == kStats || kPass == kGrad) {
-    if (p.cap > 0.0f) {
-      loss_launch_capped<kPass, true>(p, cols, s);
-      return;
+void loss_launch(const LossArgs& p, int cols, int cus, hipStream_t s) {
+  if constexpr (kPass == kWeight) {
+    loss_launch_cols<kPass, 256>(p, cus, s);
+  } else {
+    switch (cols) {
+      case 64: loss_launch_cols<kPass, 64>(p, cus, s); break;
+      case 128: loss_launch_cols<kPass, 128>(p, cus, s); break;
+      case 160: loss_launch_cols<kPass, 160>(p, cus, s); break;
+      case 192: loss_launch_cols<kPass, 192>(p, cus, s); break;
+      default: loss_launch_cols<kPass, 256>(p, cus, s);
     }
   }
-  loss_launch_capped<kPass, false>(p, cols, s);
 }
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -742,15 +837,27 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count) {
   LossPlan q{};
-  q.cols = rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+  const int cus = cu_count > 0 ? cu_count : 256;
+  q.cus = cus;
   q.v_tiles = (vocab + kRows - 1) / kRows;
+  // The columns of a tile: a stage takes the matrix cores 8 cycles a column, the
+  // LDS 768 and 3 a column (its reads by four waves and its writes), an epilogue
+  // about 80 a column; the tiles go out in rounds of a workgroup a compute unit.
+  int64_t least = INT64_MAX;
+  for (const int c : {256, 192, 160, 128, 64}) {
+    const int64_t tiles = (int64_t)q.v_tiles * ((rows + c - 1) / c);
+    const int64_t cost = (tiles + cus - 1) / cus * ((int64_t)(width / kBlock) * std::max(8 * c, 768 + 3 * c) + 80 * c);
+    if (cost < least) {
+      least = cost;
+      q.cols = c;
+    }
+  }
   // a piece: at most 256 MB of g, and its offsets (and W's) within 31 bits
   int64_t piece = ((int64_t)256 << 20) / ((int64_t)rows * 2);
   piece = std::min<int64_t>(piece, ((int64_t)1 << 30) / width - 256);
   piece = std::max<int64_t>(256, piece / 256 * 256);
   q.piece = (int32_t)std::min<int64_t>(piece, (int64_t)q.v_tiles * 256);
   const int tiles = (width + kRows - 1) / kRows * ((rows + q.cols - 1) / q.cols);
-  const int cus = cu_count > 0 ? cu_count : 256;
   q.splits = std::max(1, std::min(cus / tiles, q.piece / 256));
   q.stats_bytes = up256((size_t)q.v_tiles * rows * sizeof(float2));
   q.g_bytes = up256((size_t)rows * q.piece * 2);
@@ -773,7 +880,7 @@ void launch_lmhead_loss(const uint16_t* hidden, const uint16_t* weight, const in
   p.row_tiles = plan.v_tiles;
   p.col_tiles = (rows + plan.cols - 1) / plan.cols;
   p.splits = 1;
-  loss_launch<kStats>(p, plan.cols, s);
+  loss_launch<kStats>(p, plan.cols, plan.cus, s);
   loss_join_kernel<<<dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(256), 0, s>>>(
       p.stats, plan.v_tiles, hidden, weight, targets, rows, width, vocab, softcap, loss, lse);
 }
@@ -786,7 +893,8 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
   uint16_t* scored = (uint16_t*)(work + plan.g_bytes);
   float* part = (float*)(work + plan.g_bytes + plan.h_bytes);
   float* most = (float*)(work + plan.g_bytes + plan.h_bytes + plan.part_bytes);
-  loss_scale_kernel<<<dim3(1), dim3(1024), 0, s>>>(dloss, targets, rows, vocab, most);
+  Column* columns = (Column*)(most + 64);
+  loss_columns_kernel<<<dim3(1), dim3(1024), 0, s>>>(dloss, targets, lse, rows, vocab, most, columns);
   if (dweight) loss_rows_kernel<<<per8, block, 0, s>>>(hidden, targets, vocab, width, n, scored);
   const int k_tiles = (width + kRows - 1) / kRows;
   int splits = 1;
@@ -795,9 +903,7 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
     p.W = weight + (size_t)v * width;
     p.H = hidden;
     p.G = (uint16_t*)work;
-    p.targets = targets;
-    p.lse = lse;
-    p.dloss = dloss;
+    p.columns = columns;
     p.most = most;
     p.part = part;
     p.cap = softcap;
@@ -805,12 +911,11 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
     p.D = width;
     p.V = std::min(plan.piece, vocab - v);
     p.v_base = v;
-    p.vocab = vocab;
     p.g_stride = (p.V + 255) / 256 * 256;
     p.row_tiles = p.g_stride / 256;
     p.col_tiles = (rows + plan.cols - 1) / plan.cols;
     p.splits = 1;
-    loss_launch<kGrad>(p, plan.cols, s);
+    loss_launch<kGrad>(p, plan.cols, plan.cus, s);
     if (dhidden) {
       // every piece fills the same shares: the last, shorter one in shorter runs
       p.row_tiles = k_tiles;
@@ -818,7 +923,7 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
       p.splits = splits;
       p.split_rows = ((p.V + splits - 1) / splits + kBlock - 1) / kBlock * kBlock;
       p.accumulate = v > 0;
-      loss_launch<kHidden>(p, plan.cols, s);
+      loss_launch<kHidden>(p, plan.cols, plan.cus, s);
     }
     if (dweight) {
       p.H = scored;
@@ -826,7 +931,7 @@ void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, con
       p.row_tiles = k_tiles;
       p.col_tiles = p.g_stride / 256;
       p.splits = 1;
-      loss_launch<kWeight>(p, 256, s);
+      loss_launch<kWeight>(p, 256, plan.cus, s);
     }
   }
   if (dhidden) loss_hidden_kernel<<<per8, block, 0, s>>>(part, splits, n, targets, most, vocab, width, dhidden);
