@@ -174,11 +174,14 @@ int ensure_fused(gs_context* ctx, int32_t rows) {
   return GS_OK;
 }
 
-// The calling thread's current device, put back at the end of a call.
+// Makes the context's device the calling thread's current one for a call.
 struct DeviceGuard {
   int before = -1;
-  DeviceGuard() {
-    if (hipGetDevice(&before) != hipSuccess) before = -1;
+  hipError_t error = hipSuccess;
+  explicit DeviceGuard(const gs_context* ctx) {
+    error = hipGetDevice(&before);
+    if (error != hipSuccess || before == ctx->device) before = -1;
+    if (error == hipSuccess && before >= 0) error = hipSetDevice(ctx->device);
   }
   ~DeviceGuard() {
     if (before >= 0) (void)hipSetDevice(before);
@@ -1184,8 +1187,8 @@ int gs_rms_norm(gs_context* ctx, const void* x, const void* residual, const void
       ((uintptr_t)weight & (weight_dtype == GS_BF16 ? 1 : 3)))
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
   if (codes && !aligned16(codes)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes must be 16-byte aligned");
-  DeviceGuard guard;
-  GS_HIP(ctx, hipSetDevice(ctx->device));
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   NormArgs a{};
   a.x = x;
   a.residual = residual;
@@ -1214,11 +1217,11 @@ int gs_rms_norm_grad(gs_context* ctx, const void* dy, const void* h, const void*
   if (!bad && rows && !dx && !dweight) bad = "no output is given";
   if (bad) return fail(ctx, GS_ERR_INVALID_ARGUMENT, bad);
   if (width > kNormMaxWidth) return fail(ctx, GS_ERR_UNSUPPORTED, "rms_norm width must be at most 16384");
-  DeviceGuard guard;
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   hipStream_t s = pick_stream(ctx, stream);
   if (rows == 0) {
     if (!dweight) return GS_OK;
-    GS_HIP(ctx, hipSetDevice(ctx->device));
     launch_fill_zero(dweight, (int64_t)width * 4, s);
     GS_HIP(ctx, hipGetLastError());
     return GS_OK;
@@ -1230,7 +1233,6 @@ int gs_rms_norm_grad(gs_context* ctx, const void* dy, const void* h, const void*
   if (((uintptr_t)dy | (uintptr_t)h | (uintptr_t)dsummed | (uintptr_t)dx) & mask ||
       ((uintptr_t)weight & (weight_dtype == GS_BF16 ? 1 : 3)) || ((uintptr_t)dweight & 3))
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "rows must be aligned to their elements");
-  GS_HIP(ctx, hipSetDevice(ctx->device));
   if (dweight) {
     const int st = ensure_work(ctx, (size_t)norm_parts(rows, width) * width * sizeof(float), s);
     if (st != GS_OK) return st;
@@ -1266,8 +1268,8 @@ int gs_mx_quantize(gs_context* ctx, const void* x, int32_t dtype, int32_t format
   if (rows > 1 && row_stride < width) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "row_stride is smaller than the width");
   if (((uintptr_t)x & (dtype == GS_BF16 ? 1 : 3)) || !aligned16(codes))
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "x must be aligned to its elements, codes to 16 bytes");
-  DeviceGuard guard;
-  GS_HIP(ctx, hipSetDevice(ctx->device));
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   launch_mx_quantize(x, dtype == GS_BF16, format, rows, width, row_stride, codes, scales, pick_stream(ctx, stream));
   GS_HIP(ctx, hipGetLastError());
   return GS_OK;
@@ -1282,8 +1284,8 @@ int gs_mx_dequantize(gs_context* ctx, const uint8_t* codes, const uint8_t* scale
   if (rows == 0) return GS_OK;
   if (!codes || !scales || !out) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes, scales and out are required");
   if (!aligned16(codes) || !aligned16(out)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "codes and out must be 16-byte aligned");
-  DeviceGuard guard;
-  GS_HIP(ctx, hipSetDevice(ctx->device));
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   launch_mx_dequantize(codes, scales, format, rows, width, dtype == GS_BF16, out, pick_stream(ctx, stream));
   GS_HIP(ctx, hipGetLastError());
   return GS_OK;
@@ -1305,8 +1307,8 @@ int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hi
   if (((uintptr_t)hidden_scales | (uintptr_t)weight_scales) & 1)
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "scales must be 2-byte aligned");
   if ((uintptr_t)logits & 3) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "logits must be aligned to their elements");
-  DeviceGuard guard;
-  GS_HIP(ctx, hipSetDevice(ctx->device));
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   const int32_t slot = timing_slot(ctx);
   launch_mx_lmhead(hidden_codes, hidden_scales, weight_codes, weight_scales, m_rows, width, ctx->vocab, softcap, logits,
                    pick_stream(ctx, stream), stage_events(ctx, slot, GS_STAGE_LMHEAD));
@@ -1337,8 +1339,8 @@ int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, cons
   if (!aligned16(hidden) || !aligned16(weight)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden and weight must be 16-byte aligned");
   if (((uintptr_t)targets | (uintptr_t)loss | (uintptr_t)lse) & 3)
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "targets, loss and lse must be aligned to their elements");
-  DeviceGuard guard;
-  GS_HIP(ctx, hipSetDevice(ctx->device));
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   hipStream_t s = pick_stream(ctx, stream);
   const LossPlan plan = loss_plan(rows, width, ctx->vocab, ctx->cu_count);
   st = ensure_work(ctx, plan.stats_bytes, s);
@@ -1357,11 +1359,11 @@ int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight,
   if (rows && !dhidden && !dweight) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "no output is given");
   if (!aligned16(dhidden) || !aligned16(dweight))
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "dhidden and dweight must be 16-byte aligned");
-  DeviceGuard guard;
+  DeviceGuard guard(ctx);
+  GS_HIP(ctx, guard.error);
   hipStream_t s = pick_stream(ctx, stream);
   if (rows == 0) {
     if (!dweight) return GS_OK;
-    GS_HIP(ctx, hipSetDevice(ctx->device));
     launch_fill_zero(dweight, (int64_t)ctx->vocab * width * 2, s);
     GS_HIP(ctx, hipGetLastError());
     return GS_OK;
@@ -1371,7 +1373,6 @@ int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight,
   if (!aligned16(hidden) || !aligned16(weight)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden and weight must be 16-byte aligned");
   if (((uintptr_t)targets | (uintptr_t)lse | (uintptr_t)dloss) & 3)
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "targets, lse and dloss must be aligned to their elements");
-  GS_HIP(ctx, hipSetDevice(ctx->device));
   const LossPlan plan = loss_plan(rows, width, ctx->vocab, ctx->cu_count);
   st = ensure_work(ctx, plan.g_bytes + plan.h_bytes + plan.part_bytes + 256 + (size_t)rows * 16, s);
   if (st != GS_OK) return st;

@@ -20,6 +20,44 @@ typedef uint32_t MxU32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes at any element's alignment (rows of odd strides)
 typedef uint32_t MxU32x4Any __attribute__((ext_vector_type(4), aligned(2)));
 
+// 8 values of a row as they lie in memory (bf16: 16 bytes), to be widened later.
+template <bool kBf16>
+struct Raw8 {
+  uint32_t w[kBf16 ? 4 : 8];
+  __device__ __forceinline__ void load(const void* p, int64_t e, int n) {
+    if (kBf16) {
+      const uint16_t* q = (const uint16_t*)p + e;
+      if (n >= 8) {
+        const MxU32x4Any u = *(const MxU32x4Any*)q;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = u[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          w[i] = (2 * i < n ? (uint32_t)q[2 * i] : 0u) | (2 * i + 1 < n ? (uint32_t)q[2 * i + 1] << 16 : 0u);
+      }
+    } else {
+      const uint32_t* q = (const uint32_t*)p + e;
+      typedef uint32_t U32x4Any __attribute__((ext_vector_type(4), aligned(4)));
+      if (n >= 8) {
+        const U32x4Any a = *(const U32x4Any*)q, b = *(const U32x4Any*)(q + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = a[i];
+          w[kBf16 ? 0 : 4 + i] = b[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[kBf16 ? 0 : i] = i < n ? q[i] : 0u;
+      }
+    }
+  }
+  __device__ __forceinline__ float operator[](int i) const {
+    if (!kBf16) return __uint_as_float(w[i]);
+    return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  }
+};
+
 // 8 values of a row from element `e` on, `n` of them inside the row (zeros past it).
 template <bool kBf16>
 __device__ __forceinline__ void load_8(const void* p, int64_t e, int n, float (&v)[8]) {
@@ -115,12 +153,8 @@ __device__ __forceinline__ uint32_t mx_block_amax(const float (&v)[8]) {
     const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
     m = b > m ? b : m;
   }
-#pragma unroll
-  for (int d = 1; d < 4; d <<= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
-    m = o > m ? o : m;
-  }
-  return m;
+  m = op_max_u32(m, dpp_u32<kDppQuad1032, 0xF>(0u, m));
+  return op_max_u32(m, dpp_u32<kDppQuad2301, 0xF>(0u, m));
 }
 
 // 8 values at the block's scale as e4m3 codes (a special block: NaN codes).

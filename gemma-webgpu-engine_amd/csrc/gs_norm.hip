@@ -20,23 +20,29 @@ namespace {
 constexpr int kNormThreads = 256;
 constexpr int64_t kNormGrid = 1 << 20;  // workgroups a launch; they take more rows in turn
 
+__device__ __forceinline__ uint32_t op_add_f32(uint32_t a, uint32_t b) {
+  return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+}
+__device__ __forceinline__ float wave_sum_f32(float x) {
+  uint32_t v = __float_as_uint(x);
+  GS_WAVE_REDUCE(uint32_t, dpp_u32, v, 0u, op_add_f32);
+  return __uint_as_float(readlane_u32(v, 63));
+}
+
 // Sums of kCount values over kThreads threads (a wave, or the workgroup), the
-// same for every thread and the same order on every call.
+// same for every thread and the same order on every call. lds: 4 kCount floats
+// that the call before did not use.
 template <int kThreads, int kCount>
 __device__ __forceinline__ void row_sums(float (&v)[kCount], float* lds) {
 #pragma unroll
-  for (int c = 0; c < kCount; ++c) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v[c] += __shfl_xor(v[c], d);
-  }
+  for (int c = 0; c < kCount; ++c) v[c] = wave_sum_f32(v[c]);
   if (kThreads == 64) return;
   const int wave = threadIdx.x >> 6;
-  __syncthreads();  // the row before has been read
   if ((threadIdx.x & 63) == 0) {
 #pragma unroll
     for (int c = 0; c < kCount; ++c) lds[c * 4 + wave] = v[c];
   }
-  __syncthreads();
+  lds_barrier();
 #pragma unroll
   for (int c = 0; c < kCount; ++c) v[c] = (lds[c * 4] + lds[c * 4 + 1]) + (lds[c * 4 + 2] + lds[c * 4 + 3]);
 }
@@ -51,7 +57,8 @@ __device__ __forceinline__ void load_weight_8(const void* w, int bf16, int64_t e
 // kThreads threads a row (64: four rows a workgroup), kN pieces of 8 elements a thread.
 template <bool kBf16, int kThreads, int kN>
 __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
-  __shared__ float lds[4];
+  __shared__ float lds[2][4];
+  int turn = 0;
   const int t = threadIdx.x % kThreads;
   constexpr int kGroups = kNormThreads / kThreads;
   for (int64_t row = (int64_t)blockIdx.x * kGroups + threadIdx.x / kThreads; row < a.rows;
@@ -84,7 +91,8 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
         store_8<kBf16>(a.summed, out_at + e, a.width - e, h[i]);
       }
     }
-    row_sums<kThreads, 1>(ss, lds);
+    row_sums<kThreads, 1>(ss, lds[turn]);
+    turn ^= 1;
     const float r = 1.0f / sqrtf(ss[0] / (float)a.width + a.eps);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
@@ -109,9 +117,12 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_kernel(NormArgs a) {
 // by norm_join_kernel in one order.
 template <bool kBf16, int kThreads, int kN>
 __global__ __launch_bounds__(kNormThreads) void rms_norm_grad_kernel(NormGradArgs a) {
-  constexpr int kGroups = kNormThreads / kThreads;
-  __shared__ float lds[8];
-  __shared__ float joined[kGroups > 1 ? kThreads * kN * 8 : 1];
+  constexpr int kGroups = kNormThreads / kThreads, kSize = kBf16 ? 2 : 4;
+  __shared__ float lds[2][8];
+  // the weights, which wait apart from the rows' values here (a wait for one
+  // load covers all that were issued before it); later the waves' shares
+  __shared__ __attribute__((aligned(16))) float weights[kThreads * kN * 8];
+  int turn = 0;
   const int t = threadIdx.x % kThreads, group = threadIdx.x / kThreads;
   float dw[kN][8];
 #pragma unroll
@@ -119,22 +130,35 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_grad_kernel(NormGradArg
 #pragma unroll
     for (int k = 0; k < 8; ++k) dw[i][k] = 0.0f;
   }
-  for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < a.rows; row += (int64_t)gridDim.x * kGroups) {
-    const char* dy = (const char*)a.dy + row * a.dy_stride * (kBf16 ? 2 : 4);
-    const char* x = (const char*)a.h + row * a.h_stride * (kBf16 ? 2 : 4);
-    float h[kN][8], g[kN][8];
+  // The next row's values are on their way while a row is worked on, as far as
+  // the registers reach: otherwise each row waits for its own.
+  constexpr bool kAhead = kN <= (kBf16 ? 4 : 2);
+  const int64_t first = (int64_t)blockIdx.x * kGroups + group, step = (int64_t)gridDim.x * kGroups;
+  Raw8<kBf16> h[kN], g[kN], d[kN];
+  auto load = [&](int64_t row, Raw8<kBf16>(&h)[kN], Raw8<kBf16>(&g)[kN], Raw8<kBf16>(&d)[kN]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int e = (i * kThreads + t) * 8, n = a.width - e;
+      h[i].load((const char*)a.h + row * a.h_stride * kSize, e, n);
+      g[i].load((const char*)a.dy + row * a.dy_stride * kSize, e, n);
+      if (a.dsummed) d[i].load((const char*)a.dsummed + row * a.dsummed_stride * kSize, e, n);
+    }
+  };
+  if (first < a.rows) load(first, h, g, d);
+  for (int c = threadIdx.x * 8; c < kThreads * kN * 8; c += kNormThreads * 8) {
+    float w[8];
+    load_weight_8(a.weight, a.weight_bf16, c, a.width - c, a.offset, w);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) weights[c + k] = w[k];
+  }
+  lds_barrier();
+  for (int64_t row = first; row < a.rows; row += step) {
+    Raw8<kBf16> h1[kN], g1[kN], d1[kN];
+    if (kAhead && row + step < a.rows) load(row + step, h1, g1, d1);
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int e = (i * kThreads + t) * 8, n = a.width - e;
-      load_8<kBf16>(x, e, n, h[i]);
-      load_8<kBf16>(dy, e, n, g[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < kN; ++i) {
-      const int e = (i * kThreads + t) * 8, n = a.width - e;
-      float w[8];
-      load_weight_8(a.weight, a.weight_bf16, e, n, a.offset, w);
+      const float* w = &weights[(i * kThreads + t) * 8];
       float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -144,30 +168,42 @@ __global__ __launch_bounds__(kNormThreads) void rms_norm_grad_kernel(NormGradArg
       s[0] += s0;
       s[1] += s1;
     }
-    row_sums<kThreads, 2>(s, lds);
+    row_sums<kThreads, 2>(s, lds[turn]);
+    turn ^= 1;
     const float r = 1.0f / sqrtf(s[0] / (float)a.width + a.eps);
     const float c = r * r * (s[1] / (float)a.width);
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int e = (i * kThreads + t) * 8, n = a.width - e;
       if (a.dx) {
-        float w[8], d[8];
-        load_weight_8(a.weight, a.weight_bf16, e, n, a.offset, w);
-        if (a.dsummed) load_8<kBf16>((const char*)a.dsummed + row * a.dsummed_stride * (kBf16 ? 2 : 4), e, n, d);
+        const float* w = &weights[e];
+        float v[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const float v = r * (g[i][k] * w[k] - h[i][k] * c);
-          d[k] = a.dsummed ? v + d[k] : v;
+          v[k] = r * (g[i][k] * w[k] - h[i][k] * c);
+          if (a.dsummed) v[k] += d[i][k];
         }
-        store_8<kBf16>(a.dx, row * a.width + e, n, d);
+        store_8<kBf16>(a.dx, row * a.width + e, n, v);
       }
 #pragma unroll
       for (int k = 0; k < 8; ++k) dw[i][k] = __builtin_fmaf(g[i][k], h[i][k] * r, dw[i][k]);
+    }
+    if (kAhead) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        h[i] = h1[i];
+        g[i] = g1[i];
+        d[i] = d1[i];
+      }
+    } else if (row + step < a.rows) {
+      load(row + step, h, g, d);
     }
   }
   if (!a.parts) return;
   if (kGroups > 1) {
     // the waves' shares one after another
+    float* joined = weights;
+    __syncthreads();
     for (int w = 0; w < kGroups; ++w) {
       if (group == w) {
 #pragma unroll
@@ -255,10 +291,13 @@ void norm_backward(const NormGradArgs& a, hipStream_t s) {
 // Many narrow rows: a wave a row (no barrier). Few, or wide: a workgroup a row.
 bool norm_wave_rows(int32_t rows, int32_t width) { return rows >= 2048 && width <= 2048; }
 
-// Workgroups of the gradient's kernel: as many shares of dw.
+// Workgroups of the gradient's kernel: as many shares of dw. About 512, two a
+// compute unit (rows 4099, width 3840: 256 take 71 us, 1024 51, 512 49), and as
+// many rows for each as can be alike.
 int32_t norm_parts(int32_t rows, int32_t width) {
-  const int32_t groups = norm_wave_rows(rows, width) ? (rows + 3) / 4 : rows;
-  return groups < 512 ? groups : 512;
+  const int32_t groups = norm_wave_rows(rows, width) ? rows / 4 + (rows % 4 != 0) : rows;
+  const int32_t each = groups < 768 ? 1 : groups / 512 + (groups % 512 >= 256);
+  return groups / each + (groups % each != 0);
 }
 
 void launch_rms_norm(const NormArgs& a, bool bf16, hipStream_t s) {

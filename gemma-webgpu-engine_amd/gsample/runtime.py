@@ -290,12 +290,27 @@ def _csr(lists: Optional[Sequence[Sequence[int]]], rows: int):
     return offsets, ids
 
 
+# torch's float types that the library takes and their gs_dtype, known once torch is imported
+_FLOATS: tuple = ()
+_DTYPE_CODES: dict = {}
+
+
+def _torch_types():
+    import torch
+
+    global _FLOATS
+    if not _FLOATS:
+        _DTYPE_CODES.update({torch.float32: GS_F32, torch.bfloat16: GS_BF16})
+        _FLOATS = tuple(_DTYPE_CODES)
+
+
 class Sampler:
     """A libgsample context on one GPU: batched sampling, masks, lm_head."""
 
     def __init__(self, vocab_size: int = 262144, max_rows: int = 256, device: int = 0):
         import torch
 
+        _torch_types()
         self.torch = torch
         self.lib = library()
         self.vocab = int(vocab_size)
@@ -575,33 +590,35 @@ class Sampler:
         """The pointer of a checked contiguous tensor (None: NULL)."""
         if t is None:
             return None
-        dtypes = dtype if isinstance(dtype, tuple) else (dtype,)
-        if t.dtype not in dtypes:
-            raise GSampleError(1, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
-        if t.device != self.device:
-            raise GSampleError(1, f"{name} must live on the sampler's device")
-        if shape is not None and tuple(t.shape) != tuple(shape):
-            raise GSampleError(1, f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-        if not t.is_contiguous():
-            raise GSampleError(1, f"{name} must be contiguous")
-        return t.data_ptr()
+        if ((t.dtype is dtype or t.dtype in _FLOATS and dtype is _FLOATS) and t.device == self.device
+                and (shape is None or t.shape == shape) and t.is_contiguous()):
+            return t.data_ptr()
+        self._refuse(t, name, dtype, shape)
+        raise GSampleError(1, f"{name} must be contiguous")
 
     def _rows(self, t, name: str, dtype, shape=None):
         """(pointer, row stride) of a checked tensor of rows (None: NULL)."""
         if t is None:
             return None, 0
+        if ((t.dtype is dtype or t.dtype in _FLOATS and dtype is _FLOATS) and t.device == self.device
+                and t.dim() == 2 and (shape is None or t.shape == shape)):
+            stride, one = t.stride()
+            rows, width = t.shape
+            if (width <= 1 or one == 1) and (rows <= 1 or stride >= width):
+                return t.data_ptr(), stride
+        self._refuse(t, name, dtype, shape, 2)
+        raise GSampleError(1, f"{name}'s rows must be contiguous and not overlap")
+
+    def _refuse(self, t, name, dtype, shape, dims=None):
+        """Raises for a wrong type, device or shape."""
         dtypes = dtype if isinstance(dtype, tuple) else (dtype,)
         if t.dtype not in dtypes:
             raise GSampleError(1, f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}")
         if t.device != self.device:
             raise GSampleError(1, f"{name} must live on the sampler's device")
-        if t.dim() != 2 or (shape is not None and tuple(t.shape) != tuple(shape)):
+        if shape is not None and tuple(t.shape) != tuple(shape) or dims is not None and t.dim() != dims:
             raise GSampleError(1, f"{name} must have shape {tuple(shape) if shape else '(rows, width)'}, "
                                   f"not {tuple(t.shape)}")
-        rows, width = t.shape
-        if (width > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < width):
-            raise GSampleError(1, f"{name}'s rows must be contiguous and not overlap")
-        return t.data_ptr(), t.stride(0)
 
     def _empty(self, shape, dtype, stream):
         """Memory for a result of a call on `stream`: the caching allocator must
@@ -629,11 +646,10 @@ class Sampler:
         (then `out` is written too only if it is given, and the return value is
         (codes, scales)). h goes to `summed` where that is given."""
         torch = self.torch
-        kinds = (torch.float32, torch.bfloat16)
-        px, x_stride = self._rows(x, "x", kinds)
-        rows, width = (int(n) for n in x.shape)
+        px, x_stride = self._rows(x, "x", _FLOATS)
+        rows, width = x.shape
         pr, r_stride = self._rows(residual, "residual", x.dtype, (rows, width))
-        pw = self._tensor(weight, "weight", kinds, (width,))
+        pw = self._tensor(weight, "weight", _FLOATS, (width,))
         if (codes is None) != (scales is None):
             raise GSampleError(1, "codes and scales go together")
         if out is None and codes is None:
@@ -644,9 +660,8 @@ class Sampler:
         psc = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
         s = self._begin(stream)
         self._check(self.lib.gs_rms_norm(
-            self.ctx, px, pr, pw, GS_BF16 if x.dtype == torch.bfloat16 else GS_F32,
-            GS_BF16 if weight.dtype == torch.bfloat16 else GS_F32, rows, width, x_stride, r_stride, float(eps),
-            float(weight_offset), ps, po, pc, psc, s))
+            self.ctx, px, pr, pw, _DTYPE_CODES[x.dtype], _DTYPE_CODES[weight.dtype], rows, width, x_stride, r_stride,
+            eps, weight_offset, ps, po, pc, psc, s))
         self._end(stream)
         return out if codes is None else (codes, scales)
 
@@ -656,12 +671,11 @@ class Sampler:
         a residual) and, if the residual stream goes on, its gradient dsummed. dx (of dy's
         type) is the gradient of x and of the residual; dweight is f32 [width]."""
         torch = self.torch
-        kinds = (torch.float32, torch.bfloat16)
-        ph, h_stride = self._rows(summed, "summed", kinds)
-        rows, width = (int(n) for n in summed.shape)
+        ph, h_stride = self._rows(summed, "summed", _FLOATS)
+        rows, width = summed.shape
         pd, d_stride = self._rows(dy, "dy", summed.dtype, (rows, width))
         pds, ds_stride = self._rows(dsummed, "dsummed", summed.dtype, (rows, width))
-        pw = self._tensor(weight, "weight", kinds, (width,))
+        pw = self._tensor(weight, "weight", _FLOATS, (width,))
         if dx is None:
             dx = self._empty((rows, width), summed.dtype, stream)
         if dweight is None:
@@ -670,9 +684,8 @@ class Sampler:
         pdw = self._tensor(dweight, "dweight", torch.float32, (width,))
         s = self._begin(stream)
         self._check(self.lib.gs_rms_norm_grad(
-            self.ctx, pd, ph, pw, pds, GS_BF16 if summed.dtype == torch.bfloat16 else GS_F32,
-            GS_BF16 if weight.dtype == torch.bfloat16 else GS_F32, rows, width, d_stride, h_stride, ds_stride,
-            float(eps), float(weight_offset), px, pdw, s))
+            self.ctx, pd, ph, pw, pds, _DTYPE_CODES[summed.dtype], _DTYPE_CODES[weight.dtype], rows, width, d_stride,
+            h_stride, ds_stride, eps, weight_offset, px, pdw, s))
         self._end(stream)
         return dx, dweight
 
@@ -686,8 +699,8 @@ class Sampler:
         fmt "e2m1" (codes uint8 [rows][width / 2]) or "e4m3" ([rows][width])."""
         torch = self.torch
         f = self._mx_format(fmt)
-        px, x_stride = self._rows(x, "x", (torch.float32, torch.bfloat16))
-        rows, width = (int(n) for n in x.shape)
+        px, x_stride = self._rows(x, "x", _FLOATS)
+        rows, width = x.shape
         shape = (rows, width // 2 if f == GS_MX_E2M1 else width)
         if codes is None:
             codes = self._empty(shape, torch.uint8, stream)
@@ -696,8 +709,7 @@ class Sampler:
         pc = self._tensor(codes, "codes", torch.uint8, shape)
         ps = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
         s = self._begin(stream)
-        self._check(self.lib.gs_mx_quantize(self.ctx, px, GS_BF16 if x.dtype == torch.bfloat16 else GS_F32, f, rows,
-                                            width, x_stride, pc, ps, s))
+        self._check(self.lib.gs_mx_quantize(self.ctx, px, _DTYPE_CODES[x.dtype], f, rows, width, x_stride, pc, ps, s))
         self._end(stream)
         return codes, scales
 
@@ -709,14 +721,13 @@ class Sampler:
         pc = self._tensor(codes, "codes", torch.uint8)
         if codes.dim() != 2:
             raise GSampleError(1, "codes must have two dimensions")
-        rows, width = int(codes.shape[0]), int(codes.shape[1]) * (2 if f == GS_MX_E2M1 else 1)
+        rows, width = codes.shape[0], codes.shape[1] * (2 if f == GS_MX_E2M1 else 1)
         ps = self._tensor(scales, "scales", torch.uint8, (rows, width // 32))
         if out is None:
             out = self._empty((rows, width), torch.bfloat16 if dtype is None else dtype, stream)
-        po = self._tensor(out, "out", (torch.float32, torch.bfloat16), (rows, width))
+        po = self._tensor(out, "out", _FLOATS, (rows, width))
         s = self._begin(stream)
-        self._check(self.lib.gs_mx_dequantize(self.ctx, pc, ps, f, rows, width,
-                                              GS_BF16 if out.dtype == torch.bfloat16 else GS_F32, po, s))
+        self._check(self.lib.gs_mx_dequantize(self.ctx, pc, ps, f, rows, width, _DTYPE_CODES[out.dtype], po, s))
         self._end(stream)
         return out
 
@@ -726,7 +737,7 @@ class Sampler:
         ph = self._tensor(hidden, "hidden", u8)
         if hidden.dim() != 2:
             raise GSampleError(1, "hidden must have shape (rows, width)")
-        m, width = (int(n) for n in hidden.shape)
+        m, width = hidden.shape
         phs = self._tensor(hidden_scales, "hidden_scales", u8, (m, width // 32))
         pw = self._tensor(weight, "weight", u8, (self.vocab, width // 2))
         pws = self._tensor(weight_scales, "weight_scales", u8, (self.vocab, width // 32))
@@ -772,7 +783,7 @@ class Sampler:
         ph = self._tensor(hidden, "hidden", torch.bfloat16)
         if hidden.dim() != 2:
             raise GSampleError(1, "hidden must have shape (rows, width)")
-        rows, width = (int(n) for n in hidden.shape)
+        rows, width = hidden.shape
         pw = self._tensor(weight, "weight", torch.bfloat16, (self.vocab, width))
         pt = self._tensor(targets, "targets", torch.int32, (rows,))
         return ph, pw, pt, rows, width

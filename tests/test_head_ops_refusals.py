@@ -15,6 +15,7 @@ class NoLibrary:
 
 @pytest.fixture
 def sampler():
+    rt._torch_types()
     s = object.__new__(rt.Sampler)
     s.torch, s.vocab, s.device, s.ctx = torch, 128, torch.device("cpu"), None
     s.lib = NoLibrary()
