@@ -1311,7 +1311,7 @@ int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hi
   GS_HIP(ctx, guard.error);
   const int32_t slot = timing_slot(ctx);
   launch_mx_lmhead(hidden_codes, hidden_scales, weight_codes, weight_scales, m_rows, width, ctx->vocab, softcap, logits,
-                   pick_stream(ctx, stream), stage_events(ctx, slot, GS_STAGE_LMHEAD));
+                   ctx->cu_count, pick_stream(ctx, stream), stage_events(ctx, slot, GS_STAGE_LMHEAD));
   GS_HIP(ctx, hipGetLastError());
   return GS_OK;
 }

@@ -655,7 +655,7 @@ void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int32_t f
                           bool bf16, void* out, hipStream_t s);
 void launch_mx_lmhead(const uint8_t* hidden, const uint8_t* hidden_scales, const uint8_t* weight,
                       const uint8_t* weight_scales, int32_t m, int32_t width, int32_t vocab, float softcap, float* out,
-                      hipStream_t s, LaunchEvents ev = {});
+                      int32_t cu_count, hipStream_t s, LaunchEvents ev = {});
 
 // ------------------------------------------- the head's cross entropy
 struct LossPlan {

@@ -34,7 +34,6 @@ enum Pass { kStats, kGrad, kHidden, kWeight };
 constexpr int kLossThreads = 256;
 constexpr int kRows = 256;  // rows of a tile (vocabulary rows; columns of K in kHidden and kWeight)
 constexpr int kBlock = 64;  // of the summed index a stage
-constexpr float kLog2e = 1.44269504088896341f;
 constexpr float kLowest = -1.0e38f;  // a maximum over nothing; times log2(e) still finite
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -224,47 +223,6 @@ __device__ __forceinline__ void loss_columns(const LossArgs& p, int c0, int wave
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (LdsPtr)(lds + 1024 * wave), 16, (uint32_t)((c0 + 64 * wave + lane) * 16), 0, 0, 0);
 #endif
 }
-
-// The cap, x -> cap tanh(x / cap). Below 5/8 of the cap tanh q = q (1 + s P(s)),
-// s = q^2, P of degree 4 fitted over that range (relative error 2^-27); past it
-// 1 - 2 / (e^2q + 1). Either is within 2e-7 of the cap.
-__device__ constexpr float kCapP[5] = {-0x1.555532p-2f, 0x1.110726p-3f, -0x1.b83c58p-5f, 0x1.52268ep-6f, -0x1.75e194p-8f};
-__device__ __forceinline__ float cap_series(float s) {
-  float u = kCapP[4];
-#pragma unroll
-  for (int i = 3; i >= 0; --i) u = __builtin_fmaf(u, s, kCapP[i]);
-  return __builtin_fmaf(u, s, 1.0f);
-}
-__device__ __forceinline__ float cap_far(float q) {
-  return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(q * (2.0f * kLog2e)) + 1.0f);
-}
-__device__ __forceinline__ float cap_any(float q) {  // tanh q
-  return __builtin_fabsf(q) < kTanhSmall ? q * cap_series(q * q) : cap_far(q);
-}
-
-// The near part in x itself: cap tanh(x / cap) log2(e) = x u(x^2), the powers of
-// 1 / cap and log2(e) in u's coefficients. `far`: where |x| has to stay below
-// (0, never, for caps whose powers leave binary32's range).
-struct CapSeries {
-  float u[6], far;
-  __device__ __forceinline__ CapSeries(float cap) {
-    const float r = 1.0f / cap, r2 = r * r;
-    float c = kLog2e;
-    u[0] = c;
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      c *= r2;
-      u[i + 1] = kCapP[i] * c;
-    }
-    far = cap >= 0x1p-6f && cap <= 0x1p10f ? kTanhSmall * cap : 0.0f;
-  }
-  __device__ __forceinline__ float operator()(float s) const {
-    float v = u[5];
-#pragma unroll
-    for (int i = 4; i >= 0; --i) v = __builtin_fmaf(v, s, u[i]);
-    return v;
-  }
-};
 
 // A (max, sum of exponentials over it) pair with another's.
 __device__ __forceinline__ void join_sums(float& mx, float& sum, float om, float os) {
@@ -501,7 +459,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
     const int row8 = 128 * wr + 16 * (eg & 1) + 4 * (eg & 2);  // after an exchange: 8 rows from 16 a + this on, a even
     const bool tail = V - r0 < kRows;  // (uniform; kStats, kGrad) the tile ends past the vocabulary
     if constexpr (kPass == kStats) {
-      const CapSeries series(p.cap);
+      const CapSeries series(p.cap, kLog2e);
       float2* sums_of = (float2*)scratch;  // [2][kCols]
 #pragma unroll
       for (int b = 0; b < kCT; ++b) {
@@ -571,7 +529,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
       }
       lds_barrier();  // read before a fetch takes the place
     } else if constexpr (kPass == kGrad) {
-      const CapSeries series(p.cap);
+      const CapSeries series(p.cap, kLog2e);
       const float per_cap2 = 1.0f / (p.cap * kLog2e) / (p.cap * kLog2e);
       // the columns' values have landed for every wave; the next tile's fetches may be under way
       asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFive ? T::kFetchB : 8 + T::kFetchB) : "memory");

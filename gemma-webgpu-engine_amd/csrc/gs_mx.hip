@@ -1,5 +1,7 @@
 // Microscaled blocks (gs_mx.h): quantisation, reading back, and the lm_head
 // over e2m1 weights and e4m3 hidden states.
+#include <algorithm>
+
 #include "gs_cap.h"
 #include "gs_mx.h"
 
@@ -7,8 +9,9 @@ namespace gs {
 namespace {
 
 // ------------------------------------------------- values <-> codes
-// One thread 8 values, four threads a block. Memory bound: a value is read
-// once and its code and scale written once.
+// One thread 8 values, four threads a block. Memory bound: a value is read once
+// and its code and scale written once (262144 x 2048 bf16 to e2m1 and back: 559 us
+// for 2.7 GB, 4.9 TB/s, what a copy of that size reaches).
 constexpr int kMxThreads = 256;
 
 template <bool kBf16, bool kFp4>
@@ -64,8 +67,20 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t
 
 // ------------------------------------------------- the 4-bit head
 // logits[m][v] = cap(sum over blocks of 2^(sh + sw) sum_k h[m][k] w[v][k]) on
-// v_mfma_scale_f32_16x16x128_f8f6f4 (the scales are its operands), tiles of
-// 256 vocabulary rows by kCols hidden rows, 8 waves, 256 columns of K a stage.
+// v_mfma_scale_f32_16x16x128_f8f6f4 (the scales are its operands). The
+// instruction adds 8 neighbouring products in fixed point, cut 13 bits below the
+// largest of them, and the groups' sums in binary32: a group of 8 is off by at
+// most 2^-10 of its largest product, and the logits of random operands by 5e-6 of
+// their norm (a chain of binary32 sums: 1e-7). That is far below what the codes
+// themselves leave out (2^-4 and more of a value), and the exact alternative,
+// products of the codes widened to bf16, has a quarter of the rate and its own
+// conversions.
+//
+// ---- up to 64 hidden rows: bound by W's bytes
+// Tiles of 256 vocabulary rows by kCols hidden rows, 8 waves, 256 columns of K a
+// stage, three stages in LDS, two of them on the way. 1 row by 262144 x 1536: 42 us
+// for 214 MB, 5.1 TB/s; 64 rows by 262144 x 2048: 74 us for 352 MB (67 MB of them
+// logits), 4.8 TB/s; a copy reaches 5.2.
 //
 // K order: the instruction multiplies four blocks of 32 at a time, one a group
 // of 16 lanes. Step s (of two) of a stage takes blocks s, 2 + s, 4 + s, 6 + s,
@@ -85,11 +100,9 @@ typedef __attribute__((address_space(3))) void* LdsPtr;
 
 template <int kCols>
 struct HeadTile {
-  static constexpr int kWavesV = kCols == 128 ? 4 : 8;
-  static constexpr int kWavesM = 8 / kWavesV;
-  static constexpr int kRT = 16 / kWavesV;            // 16-row tiles of W a wave
-  static constexpr int kCT = kCols / 16 / kWavesM;    // 16-row tiles of H a wave
-  static constexpr int kStages = kCols == 128 ? 2 : 3;
+  static constexpr int kRT = 2;                       // 16-row tiles of W a wave (8 waves)
+  static constexpr int kCT = kCols / 16;              // 16-row tiles of H a wave
+  static constexpr int kStages = 3;
   static constexpr int kW = kHeadRows * 128;          // bytes of a stage: codes of W,
   static constexpr int kH = kCols * 256;              // of H,
   static constexpr int kWS = kHeadRows * 16;          // scales of W (a dword holds a pair),
@@ -132,15 +145,15 @@ __device__ __forceinline__ void head_fetch(char* lds, char* spare, int wave, Rsr
 // One stage: the next fetches go out, then two steps of 128 columns.
 template <int kCols, typename Rsrc>
 __device__ __forceinline__ void head_block(const char* __restrict__ cur, char* __restrict__ next, char* spare, int wave,
-                                           int wv, int wm, int j, int g, Rsrc wr, Rsrc hr, Rsrc wsr, Rsrc hsr,
+                                           int wv, int j, int g, Rsrc wr, Rsrc hr, Rsrc wsr, Rsrc hsr,
                                            const HeadOffsets& o, uint32_t k, bool tail, bool none,
                                            f32x4 (&acc)[HeadTile<kCols>::kRT][HeadTile<kCols>::kCT]) {
   typedef HeadTile<kCols> T;
   head_fetch<kCols>(next, spare, wave, wr, hr, wsr, hsr, o, k, tail, none);
   const char* w = cur + (16 * T::kRT * wv + j) * 128;
-  const char* h = cur + T::kW + (16 * T::kCT * wm + j) * 256;
+  const char* h = cur + T::kW + j * 256;
   const int* ws = (const int*)(cur + T::kW + T::kH) + (16 * T::kRT * wv + j) * 4 + g;
-  const int* hs = (const int*)(cur + T::kW + T::kH + T::kWS) + (16 * T::kCT * wm + j) * 4 + g;
+  const int* hs = (const int*)(cur + T::kW + T::kH + T::kWS) + j * 4 + g;
   int sw[T::kRT], sh[T::kCT];
 #pragma unroll
   for (int a = 0; a < T::kRT; ++a) sw[a] = ws[64 * a];
@@ -184,7 +197,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
   const int64_t v0 = (int64_t)vt * kHeadRows, m0 = (int64_t)(local % m_blocks) * kCols;
   if (v0 >= V) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4, wv = wave % T::kWavesV, wm = wave / T::kWavesV;
+  const int j = lane & 15, g = lane >> 4, wv = wave;
   const int v_rows = V - v0 < kHeadRows ? (int)(V - v0) : kHeadRows;
   const int m_rows = M - m0 < kCols ? (int)(M - m0) : kCols;
   const int ds = D / 32;
@@ -242,7 +255,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
         // the stage has landed for every wave, and every wave has read the one before
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
         const int n = kb + u + T::kStages - 1, k = at(n);
-        head_block<kCols>(lds + u * T::kStage, lds + (u + T::kStages - 1) % T::kStages * T::kStage, spare, wave, wv, wm, j,
+        head_block<kCols>(lds + u * T::kStage, lds + (u + T::kStages - 1) % T::kStages * T::kStage, spare, wave, wv, j,
                           g, wr, hr, wsr, hsr, o, (uint32_t)k, partial(k), n >= nk, acc);
       }
     }
@@ -253,14 +266,14 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
   // the cap, then the tile through LDS, so that rows go out in pieces of 1 KB
   // (lane (j, g) holds column j of H's rows, rows 4 g + e of W's)
   float* stage = (float*)lds;
-  const float rcap = reciprocal_of_cap(cap);
+  const CapSeries series(cap, 1.0f);
 #pragma unroll
   for (int b = 0; b < T::kCT; ++b) {
 #pragma unroll
     for (int a = 0; a < T::kRT; ++a) {
       float x[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-      if (cap > 0.0f) lmhead_cap<4>(x, cap, rcap);
-      *(f32x4*)&stage[(16 * (T::kCT * wm + b) + j) * kHeadStride + 16 * (T::kRT * wv + a) + 4 * g] =
+      if (cap > 0.0f) cap_logits(x, cap, series);
+      *(f32x4*)&stage[(16 * b + j) * kHeadStride + 16 * (T::kRT * wv + a) + 4 * g] =
           f32x4{x[0], x[1], x[2], x[3]};
     }
   }
@@ -278,6 +291,368 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
       if (c < v_rows) __builtin_nontemporal_store(stage[row * kHeadStride + c], &p[(size_t)row * V + c]);
     }
   }
+}
+
+// ---- many hidden rows: bound by the matrix cores and the logits' stores
+// Tiles of 256 vocabulary rows by 128 or 256 hidden rows, 4 waves of 128 by half
+// of those, one a SIMD (an LDS byte is read for the fewest products so), 128
+// columns of K a stage. A stage's operands are read into registers one stage
+// ahead, and its data are on the way two or three ahead; a workgroup takes tile
+// after tile, so that the next tile's data come while the logits go out, through
+// LDS in runs of 1 KB of a row: rows lie 4 V bytes apart, and the 64-byte pieces
+// that a wave holds of 16 of them would all go to the same memory channels.
+// 512 rows by 262144 x 2048: 293 us, 1.9 PFLOP/s; the matrix cores are busy for 43 %
+// of it and the softcap's arithmetic, which nothing runs beside, for 20 %. 8 waves
+// of 32 x 128 with 64 hidden rows a tile (the form above): 430 us; the softcap
+// before the way through LDS: 520 us (its far branch makes the compiler spill).
+constexpr int kWideThreads = 256;
+constexpr int kWideK = 128;
+constexpr int kOutCache = 2;  // non-temporal: the logits are streamed once
+
+// kQuads: a row's four scales of a stage are one dword (widths that are a
+// multiple of 128), else two pairs, a dword each.
+template <int kCols, bool kQuads>
+struct WideTile {
+  static constexpr int kCT = kCols / 32;                            // 16-row tiles of H a wave
+  static constexpr int kW = kHeadRows * 64, kH = kCols * 128;       // bytes of a stage: codes,
+  static constexpr int kWS = kHeadRows * (kQuads ? 4 : 8);          // scales
+  static constexpr int kHS = 256 * (kQuads ? 4 : 8);
+  static constexpr int kPlace = kW + kH + kWS + kHS;
+  static constexpr int kPlaces = kCols == 128 ? 4 : 3;
+  static constexpr int kOut = 32 * kHeadRows * 4;                   // staged logits: 32 hidden rows at a time, in a free place
+  static constexpr int kScales = kQuads ? 1 : 2;                    // memory instructions of a wave and stage for scales, each
+  static constexpr int kFetches = 4 + kCT + 2 * kScales;
+  static constexpr int kAhead = (kPlaces - 2) * kFetches;           // newer than the stage that has to have landed
+  static_assert(kPlaces * kPlace <= 160 * 1024 && kOut <= kPlace, "LDS of a compute unit");
+};
+
+// acc += the scaled products of an e2m1 and an e4m3 operand (scales in the low
+// bytes), in place and in this order: the compiler would run the builtin's out
+// in one go, apart from the reads between them. A tile's sums are read no sooner
+// than sums_ready() after the last of these (the compiler does not count the
+// matrix core's passes through assembly).
+__device__ __forceinline__ void add_scaled_products(f32x4& acc, const i32x4& w, const i32x8& h, int ws, int hs) {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
+               : "+a"(acc)
+               : "v"(w), "v"(h), "v"(ws), "v"(hs));
+#endif
+}
+__device__ __forceinline__ void sums_ready() {
+#ifdef __HIP_DEVICE_COMPILE__
+  asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// Waits until at most kAhead memory instructions are under way (kAheadStores
+// where a tile's stores are among them), and for every wave. The choice is in the
+// assembly: around it, it would double the stage.
+template <int kAhead, int kAheadStores>
+__device__ __forceinline__ void wide_landed(int stored) {
+  asm volatile(
+      "s_cmp_lg_u32 %0, 0\n\t"
+      "s_cbranch_scc1 .Lwide%=\n\t"
+      "s_waitcnt vmcnt(%1)\n\t"
+      ".Lwide%=:\n\t"
+      "s_waitcnt vmcnt(%2) lgkmcnt(0)\n\t"
+      "s_barrier" ::"s"(stored),
+      "n"(kAhead), "n"(kAheadStores)
+      : "memory", "scc");
+}
+
+// kPieces: 16-byte pieces of a logits row (V % 4 == 0 and aligned logits).
+template <int kCols, bool kQuads, bool kPieces>
+__global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
+    const uint8_t* __restrict__ H, const uint8_t* __restrict__ HS, const uint8_t* __restrict__ W,
+    const uint8_t* __restrict__ WS, int M, int D, int V, int row_tiles, int col_tiles, float cap,
+    float* __restrict__ out) {
+  typedef WideTile<kCols, kQuads> T;
+  constexpr int kCT = T::kCT;
+  __shared__ __attribute__((aligned(16))) char lds[T::kPlaces * T::kPlace];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int j = lane & 15, g = lane >> 4, wv = wave & 1, wm = wave >> 1;
+  const int ds = D / 32;
+  // an XCD takes a run of tiles, four row tiles by all column tiles at a time
+  const int total = row_tiles * col_tiles, run = (total + 7) / 8, step = (int)(gridDim.x >> 3);
+  int id = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+  const int id_end = ((int)(blockIdx.x & 7) + 1) * run < total ? ((int)(blockIdx.x & 7) + 1) * run : total;
+  if (id >= id_end) return;
+  auto locate = [&](int id, int& v0, int& m0) __attribute__((always_inline)) {
+    const int group = id / (4 * col_tiles) * 4, in = row_tiles - group < 4 ? row_tiles - group : 4;
+    id -= group * col_tiles;
+    const int ct = id / in;
+    v0 = (group + id - ct * in) * kHeadRows;
+    m0 = ct * kCols;
+  };
+
+  // fetched rows: chunk c of row r lands at c ^ ((r >> 1) & 3) (W, 64 bytes a row) or c ^ (r & 7) (H, 128 bytes)
+  uint32_t w_off[4], h_off[kCT], ws_off[T::kScales], hs_off[T::kScales];
+  const int nk = (D + kWideK - 1) / kWideK, last_k = D - (nk - 1) * kWideK;
+  const int wc = (lane & 3) ^ ((lane >> 3) & 3), hc = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w_off[i] = (uint32_t)((64 * wave + 16 * i + (lane >> 2)) * (D / 2) + 16 * wc);
+#pragma unroll
+  for (int i = 0; i < kCT; ++i) h_off[i] = (uint32_t)((kCols / 4 * wave + 8 * i + (lane >> 3)) * D + 16 * hc);
+#pragma unroll
+  for (int i = 0; i < T::kScales; ++i) {
+    const int row = kQuads ? 64 * wave + lane : 64 * wave + 32 * i + (lane >> 1);  // (H's past kCols: nothing)
+    ws_off[i] = (uint32_t)(row * ds + (kQuads ? 0 : 2 * (lane & 1)));
+    hs_off[i] = row < kCols ? ws_off[i] : kBufferOutOfRange;
+  }
+  // without kQuads the last stage has half the columns
+  [[maybe_unused]] const uint32_t w_tail = 32 * wc < last_k ? 0u : kBufferOutOfRange;
+  [[maybe_unused]] const uint32_t h_tail = 16 * hc < last_k ? 0u : kBufferOutOfRange;
+  [[maybe_unused]] const uint32_t s_tail = 64 * (lane & 1) < last_k ? 0u : kBufferOutOfRange;
+  [[maybe_unused]] __amdgpu_buffer_rsrc_t wr, hr, wsr, hsr;
+  int f_id = id, f_left = 0, f_k = 0;
+  auto fetch_tile = [&]() __attribute__((always_inline)) {
+    int t = f_id;
+    asm volatile("" : "+s"(t));  // (nothing of this is computed ahead of the branch here)
+    int v0 = 0, m0 = 0, v_rows = 0, m_rows = 0;  // past the last tile: nothing is read
+    if (t < id_end) {
+      locate(t, v0, m0);
+      v_rows = V - v0 < kHeadRows ? V - v0 : kHeadRows;
+      m_rows = M - m0 < kCols ? M - m0 : kCols;
+    }
+    wr = __builtin_amdgcn_make_buffer_rsrc((void*)(W + (size_t)v0 * (D / 2)), (short)0, v_rows * (D / 2), kBufferWord3);
+    hr = __builtin_amdgcn_make_buffer_rsrc((void*)(H + (size_t)m0 * D), (short)0, m_rows * D, kBufferWord3);
+    wsr = __builtin_amdgcn_make_buffer_rsrc((void*)(WS + (size_t)v0 * ds), (short)0, v_rows * ds, kBufferWord3);
+    hsr = __builtin_amdgcn_make_buffer_rsrc((void*)(HS + (size_t)m0 * ds), (short)0, m_rows * ds, kBufferWord3);
+    f_left = nk;
+    f_k = v0 / kHeadRows % nk;  // tiles of W start at other columns: their reads spread over the memory channels
+  };
+  auto fetch_next = [&]() __attribute__((always_inline)) {
+    if (--f_left == 0) {
+      f_id = f_id < id_end ? f_id + step : f_id;
+      fetch_tile();
+    } else {
+      f_k = f_k + 1 < nk ? f_k + 1 : 0;
+    }
+  };
+  auto fetch = [&](int i, char* place) __attribute__((always_inline)) {  // instruction i of the stage's kFetches
+#ifdef __HIP_DEVICE_COMPILE__
+    const uint32_t part = !kQuads && f_k == nk - 1 ? ~0u : 0u;
+    char* scales = place + T::kW + T::kH;
+    if (i < 4)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (LdsPtr)(place + 4096 * wave + 1024 * i), 16, w_off[i & 3] | (part & w_tail),
+                                               (uint32_t)f_k * 64, 0, 0);
+    else if (i < 4 + kCT)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(hr, (LdsPtr)(place + T::kW + T::kH / 4 * wave + 1024 * (i - 4)), 16,
+                                               h_off[(i - 4) % kCT] | (part & h_tail), (uint32_t)f_k * 128, 0, 0);
+    else if (kQuads)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(i == 4 + kCT ? wsr : hsr, (LdsPtr)(scales + (i - 4 - kCT) * T::kWS + 256 * wave), 4,
+                                               i == 4 + kCT ? ws_off[0] : hs_off[0], (uint32_t)f_k * 4, 0, 0);
+    else if (i < 6 + kCT)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(wsr, (LdsPtr)(scales + 512 * wave + 256 * (i - 4 - kCT)), 2,
+                                               ws_off[(i - 4 - kCT) % T::kScales] | (part & s_tail), (uint32_t)f_k * 4, 0, 0);
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(hsr, (LdsPtr)(scales + T::kWS + 512 * wave + 256 * (i - 6 - kCT)), 2,
+                                               hs_off[(i - 6 - kCT) % T::kScales] | (part & s_tail), (uint32_t)f_k * 4, 0, 0);
+#endif
+  };
+
+  // reads: lane (j, g) holds block g of row j of a W tile; the halves of blocks of H's rows as the instruction deals
+  // them (columns 16 g .. and 64 + 16 g ..); the byte of block g of the rows' scales
+  const uint32_t w_pos = (uint32_t)((128 * wv + j) * 64 + ((g ^ ((j >> 1) & 3)) * 16));
+  const uint32_t h_pos0 = (uint32_t)(T::kW + (16 * kCT * wm + j) * 128 + ((g ^ (j & 7)) * 16)), h_pos1 = h_pos0 ^ 64u;
+  constexpr int kScaleRow = kQuads ? 4 : 8;
+  const uint32_t ws_pos = (uint32_t)(T::kW + T::kH + (128 * wv + j) * kScaleRow + (kQuads ? 0 : (g >> 1) * 4));
+  const uint32_t hs_pos = (uint32_t)(T::kW + T::kH + T::kWS + (16 * kCT * wm + j) * kScaleRow + (kQuads ? 0 : (g >> 1) * 4));
+  const int shift = 8 * (kQuads ? g : g & 1);
+  i32x4 w[8];
+  int ws[8];
+  // one stage: its products, and between them the next stage's reads (H's first, a row tile of W's as soon as its
+  // products are out, into its place) and the fetches of a later one
+  auto read_w = [&](const char* p, int a) __attribute__((always_inline)) {
+    w[a] = *(const i32x4*)(p + w_pos + 1024 * a);
+    ws[a] = *(const int*)(p + ws_pos + 16 * kScaleRow * a);
+  };
+  auto read_h = [&](const char* p, i32x8(&h)[kCT], int(&hs)[kCT], int b) __attribute__((always_inline)) {
+    const i32x4 lo = *(const i32x4*)(p + h_pos0 + 2048 * b), hi = *(const i32x4*)(p + h_pos1 + 2048 * b);
+    h[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    hs[b] = *(const int*)(p + hs_pos + 16 * kScaleRow * b);
+  };
+  auto stage = [&](const i32x8(&h)[kCT], const int(&hs_raw)[kCT], i32x8(&h_next)[kCT], int(&hs_next)[kCT], const char* read,
+                   char* free_place, f32x4(&acc)[8][kCT]) __attribute__((always_inline)) {
+    constexpr int kSlots = 4 * kCT;
+    int hs[kCT];
+#pragma unroll
+    for (int b = 0; b < kCT; ++b) hs[b] = hs_raw[b] >> shift;
+#pragma unroll
+    for (int t = 0; t < kSlots; ++t) {
+      if (t % 3 == 0 && t / 3 < kCT) read_h(read, h_next, hs_next, t / 3);
+      if (t > 0 && 2 * t % kCT == 0) read_w(read, 2 * t / kCT - 1);
+#pragma unroll
+      for (int i = (t * T::kFetches + kSlots - 1) / kSlots; i < ((t + 1) * T::kFetches + kSlots - 1) / kSlots; ++i)
+        fetch(i, free_place);
+#ifdef __HIP_DEVICE_COMPILE__
+      __builtin_amdgcn_sched_barrier(0x6);
+#endif
+#pragma unroll
+      for (int q = 2 * t; q < 2 * t + 2; ++q)
+        add_scaled_products(acc[q / kCT][q % kCT], w[q / kCT], h[q % kCT], ws[q / kCT] >> shift, hs[q % kCT]);
+#ifdef __HIP_DEVICE_COMPILE__
+      __builtin_amdgcn_sched_barrier(0x6);
+#endif
+    }
+    read_w(read, 7);
+  };
+
+  fetch_tile();
+  int ring[T::kPlaces];
+#pragma unroll
+  for (int u = 0; u < T::kPlaces; ++u) {
+    ring[u] = u * T::kPlace;
+#pragma unroll
+    for (int i = 0; i < T::kFetches; ++i) fetch(i, lds + u * T::kPlace);
+    fetch_next();
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kAhead) : "memory");
+  i32x8 h0[kCT], h1[kCT];
+  int hs0[kCT], hs1[kCT];
+#pragma unroll
+  for (int b = 0; b < kCT; ++b) read_h(lds, h0, hs0, b);
+#pragma unroll
+  for (int a = 0; a < 8; ++a) read_w(lds, a);
+  // (the first place is read by every wave before it is fetched into)
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  int stored = 0;  // stages to come whose wait need not cover the stores of a tile
+  const CapSeries series(cap, 1.0f);
+  const float reach = series.far * series.far * (1.0f - 0x1p-20f);  // a square below it: |x| < series.far
+  for (; id < id_end; id += step) {
+    f32x4 acc[8][kCT];
+#pragma unroll
+    for (int a = 0; a < 8; ++a) {
+#pragma unroll
+      for (int b = 0; b < kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    auto next_stage = [&]() __attribute__((always_inline)) {
+      // the stage after the next has landed for every wave, and every wave has read the next one
+      constexpr int kStores = kPieces ? 8 * kCT : 32 * kCT, kBoth = T::kAhead + kStores;
+      wide_landed<T::kAhead, kBoth < 63 ? kBoth : 63>(stored);
+      fetch_next();
+      const int r = ring[0];
+#pragma unroll
+      for (int u = 0; u + 1 < T::kPlaces; ++u) ring[u] = ring[u + 1];
+      ring[T::kPlaces - 1] = r;
+      asm volatile("s_sub_u32 %0, %0, 1\n\ts_cselect_b32 %0, 0, %0" : "+s"(stored)::"scc");  // (down to 0)
+    };
+    int kb = 0;
+    for (; kb + 1 < nk; kb += 2) {
+      stage(h0, hs0, h1, hs1, lds + ring[1], lds + ring[0], acc);
+      next_stage();
+      stage(h1, hs1, h0, hs0, lds + ring[1], lds + ring[0], acc);
+      next_stage();
+    }
+    if (kb < nk) {
+      stage(h0, hs0, h1, hs1, lds + ring[1], lds + ring[0], acc);
+      next_stage();
+#pragma unroll
+      for (int b = 0; b < kCT; ++b) {
+        h0[b] = h1[b];
+        hs0[b] = hs1[b];
+      }
+    }
+    sums_ready();
+    // lane (j, g) holds column j of H's rows, rows 4 g + e of W's
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (what follows is computed here, not kept in registers over the products)
+    const int ej = l & 15, eg = l >> 4;
+    int v0, m0;
+    locate(id, v0, m0);
+    const int m_rows = M - m0 < kCols ? M - m0 : kCols;
+    const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(out + (size_t)m0 * V + v0), (short)0, (int)(((int64_t)m_rows * V - v0) * 4), kBufferWord3);
+    // The next stage's place is free until its fetches: its operands are in registers, and every wave's reads of it
+    // are done. 16-byte piece c of staged row r lies at piece c ^ (r & 15): the lanes of a write hit different banks.
+    // The softcap comes after the way through LDS, where the values are not bound to the sums' registers.
+    char* stage_out = lds + ring[0];
+    auto store_row = [&](int r, int row, const float (&x)[4]) __attribute__((always_inline)) {
+      if (kPieces) {
+        const f32x4 y{x[0], x[1], x[2], x[3]};
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(MxU32x4, y), rows,
+                                               v0 + 4 * l < V ? (uint32_t)(row * V + 4 * l) * 4u : kBufferOutOfRange, 0, kOutCache);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x[e]), rows,
+                                                v0 + 64 * e + l < V ? (uint32_t)(row * V + 64 * e + l) * 4u : kBufferOutOfRange, 0, kOutCache);
+      }
+    };
+    auto load_row = [&](int r, float (&x)[4]) __attribute__((always_inline)) {
+      if (kPieces) {
+        const f32x4 y = *(const f32x4*)(stage_out + r * 1024 + ((l ^ (r & 15)) * 16));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = y[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = 64 * e + l;
+          x[e] = *(const float*)(stage_out + r * 1024 + (((v >> 2) ^ (r & 15)) * 16) + 4 * (v & 3));
+        }
+      }
+    };
+#pragma unroll
+    for (int b = 0; b < kCT; ++b) {
+#pragma unroll
+      for (int a = 0; a < 8; ++a)
+        *(f32x4*)(stage_out + (16 * wm + ej) * 1024 + (((32 * wv + 4 * a + eg) ^ ej) * 16)) = acc[a][b];
+      lds_barrier();
+      float x[8][4], square[8][4], largest = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        load_row(8 * wave + i, x[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          square[i][e] = x[i][e] * x[i][e];
+          largest = __builtin_fmaxf(largest, square[i][e]);  // (passes by NaN, which the series keeps)
+        }
+      }
+      auto row_of = [&](int r) { return 16 * kCT * (r >> 4) + 16 * b + (r & 15); };  // of the tile
+      if (cap <= 0.0f) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) store_row(8 * wave + i, row_of(8 * wave + i), x[i]);
+      } else if (__all(largest < reach)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i][e] *= series(square[i][e]);
+          store_row(8 * wave + i, row_of(8 * wave + i), x[i]);
+        }
+      } else {
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+          float y[4];
+          load_row(8 * wave + i, y);
+          cap_logits(y, cap, series);
+          store_row(8 * wave + i, row_of(8 * wave + i), y);
+        }
+      }
+      lds_barrier();  // read before the next rows take the place
+    }
+    stored = T::kPlaces - 2;
+  }
+  // no fetch is under way to LDS that the next workgroup may get
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <int kCols>
+void wide_launch(const uint8_t* H, const uint8_t* HS, const uint8_t* W, const uint8_t* WS, int32_t m, int32_t width,
+                 int32_t vocab, float cap, float* out, int32_t cu_count, hipStream_t s, LaunchEvents ev) {
+  const int row_tiles = (vocab + kHeadRows - 1) / kHeadRows, col_tiles = (m + kCols - 1) / kCols;
+  const int cus = cu_count > 0 ? cu_count : 256;
+  const dim3 grid((unsigned)std::min((row_tiles * col_tiles + 7) / 8 * 8, std::max(8, cus / 8 * 8))), block(kWideThreads);
+  const bool quads = width % 128 == 0 && (((uintptr_t)HS | (uintptr_t)WS) & 3) == 0;
+  const bool pieces = vocab % 4 == 0 && ((uintptr_t)out & 15) == 0;
+#define GS_CASE(q, p)                                                                                                     \
+  hipExtLaunchKernelGGL((mx_head_wide_kernel<kCols, q, p>), grid, block, 0, s, ev.start, ev.stop, 0, H, HS, W, WS, m,     \
+                        width, vocab, row_tiles, col_tiles, cap, out)
+  if (quads && pieces) GS_CASE(true, true);
+  else if (quads) GS_CASE(true, false);
+  else if (pieces) GS_CASE(false, true);
+  else GS_CASE(false, false);
+#undef GS_CASE
 }
 
 template <int kCols>
@@ -327,12 +702,24 @@ void launch_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int32_t f
 #undef GS_CASE
 }
 
+// Whether tiles have 128 hidden rows. A tile of 256 costs about 5/3 of one of 128,
+// so 128 where at most half of a tile's rows are left (W of 262144 x 2048: 118 us
+// against 156 at 128 rows, 226 against 262 at 300; 185 against 162 at 200 rows, 300
+// against 270 at 385), and where tiles of 256 would leave half of the compute units
+// without one (W of 32000 x 1152, 200 rows: 38.5 us against 46).
+bool wide_narrow(int32_t m, int32_t vocab, int32_t cu_count) {
+  const int64_t tiles = (int64_t)((vocab + kHeadRows - 1) / kHeadRows) * ((m + 255) / 256);
+  return (m <= 384 && (m - 1) % 256 < 128) || 2 * tiles <= (cu_count > 0 ? cu_count : 256);
+}
+
 void launch_mx_lmhead(const uint8_t* hidden, const uint8_t* hidden_scales, const uint8_t* weight,
                       const uint8_t* weight_scales, int32_t m, int32_t width, int32_t vocab, float softcap, float* out,
-                      hipStream_t s, LaunchEvents ev) {
+                      int32_t cu_count, hipStream_t s, LaunchEvents ev) {
   if (m <= 32) head_launch<32>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, s, ev);
   else if (m <= 64) head_launch<64>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, s, ev);
-  else head_launch<128>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, s, ev);
+  else if (wide_narrow(m, vocab, cu_count))
+    wide_launch<128>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
+  else wide_launch<256>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
 }
 
 }  // namespace gs

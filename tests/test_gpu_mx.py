@@ -161,6 +161,36 @@ def test_head_of_a_large_vocabulary_and_wide_rows(samplers):
         check_logits(samplers(vocab).mx_lmhead(*ops), hv, wv, 0.0)
 
 
+@pytest.mark.parametrize("m,width,vocab,cap,shift", [
+    (100, 64, 66001, 0.0, 0),   # tiles of 128 hidden rows, more tiles than compute units
+    (330, 192, 33000, 30.0, 0),
+    (160, 64, 33001, 30.0, 0),  # tiles of 256
+    (256, 128, 32772, 2.0, 0),
+    (250, 128, 32772, 0.0, 1),  # (logits and scales that allow no wide accesses)
+    (900, 192, 8450, 0.0, 0),
+    (600, 128, 33001, 0.5, 0),  # and more of them than compute units
+])
+def test_head_of_many_tiles(samplers, m, width, vocab, cap, shift):
+    rng = np.random.default_rng(m + width)
+    (hc, hs, wc, ws), hv, wv = head_operands(rng, m, width, vocab)
+    s = samplers(vocab)
+    out = torch.full(((m + 1) * vocab + shift,), 77.0).cuda()[shift:].view(m + 1, vocab)
+    if shift:
+        hs, ws = (torch.cat([torch.zeros(2, dtype=torch.uint8).cuda(), t.flatten()])[2:].view(t.shape) for t in (hs, ws))
+    s.mx_lmhead(hc, hs, wc, ws, softcap_value=cap, out=out[:m])
+    some = torch.from_numpy(np.unique(np.concatenate([rng.integers(0, vocab, 500), np.arange(vocab - 300, vocab)])))
+    check_logits(out[:m][:, some.cuda()], hv, wv[some], cap)
+    assert (out[m] == 77.0).all()
+    # the rest: the same sums, whatever rows a call has
+    for r in range(0, m, 120):
+        n = min(120, m - r)
+        few = s.mx_lmhead(hc[r:r + n], hs[r:r + n].contiguous(), wc, ws, softcap_value=cap)
+        if n > 64:
+            assert torch.equal(out[r:r + n], few)
+        else:
+            assert ((out[r:r + n] - few).abs() <= 1e-3 * (1 + few.abs())).all()
+
+
 def test_a_special_block_stays_in_its_own_logit(samplers):
     rng = np.random.default_rng(12)
     for width in (64, 320, 512):
