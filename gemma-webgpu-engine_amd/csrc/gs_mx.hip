@@ -299,7 +299,7 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
 // columns of K a stage. A stage's operands are read into registers one stage
 // ahead, and its data are on the way two or three ahead; a workgroup takes tile
 // after tile, so that the next tile's data come while the logits go out, through
-// LDS in runs of 1 KB of a row: rows lie 4 V bytes apart, and the 64-byte pieces
+// LDS in runs of 512 bytes of a row: rows lie 4 V bytes apart, and the 64-byte pieces
 // that a wave holds of 16 of them would all go to the same memory channels.
 // 512 rows by 262144 x 2048: 293 us, 1.9 PFLOP/s; the matrix cores are busy for 43 %
 // of it and the softcap's arithmetic, which nothing runs beside, for 20 %. 8 waves
@@ -319,7 +319,7 @@ struct WideTile {
   static constexpr int kHS = 256 * (kQuads ? 4 : 8);
   static constexpr int kPlace = kW + kH + kWS + kHS;
   static constexpr int kPlaces = kCols == 128 ? 4 : 3;
-  static constexpr int kOut = 32 * kHeadRows * 4;                   // staged logits: 32 hidden rows at a time, in a free place
+  static constexpr int kOut = 32 * kHeadRows * 4;                   // staged logits: 16 hidden rows a wave, in a free place
   static constexpr int kScales = kQuads ? 1 : 2;                    // memory instructions of a wave and stage for scales, each
   static constexpr int kFetches = 4 + kCT + 2 * kScales;
   static constexpr int kAhead = (kPlaces - 2) * kFetches;           // newer than the stage that has to have landed
@@ -359,6 +359,14 @@ __device__ __forceinline__ void wide_landed(int stored) {
       "s_barrier" ::"s"(stored),
       "n"(kAhead), "n"(kAheadStores)
       : "memory", "scc");
+}
+
+// LDS accesses of a wave on both sides stay on their sides (it runs them in order).
+__device__ __forceinline__ void wave_order() {
+#ifdef __HIP_DEVICE_COMPILE__
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#endif
 }
 
 // kPieces: 16-byte pieces of a logits row (V % 4 == 0 and aligned logits).
@@ -460,43 +468,60 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
   const uint32_t ws_pos = (uint32_t)(T::kW + T::kH + (128 * wv + j) * kScaleRow + (kQuads ? 0 : (g >> 1) * 4));
   const uint32_t hs_pos = (uint32_t)(T::kW + T::kH + T::kWS + (16 * kCT * wm + j) * kScaleRow + (kQuads ? 0 : (g >> 1) * 4));
   const int shift = 8 * (kQuads ? g : g & 1);
-  i32x4 w[8];
-  int ws[8];
-  // one stage: its products, and between them the next stage's reads (H's first, a row tile of W's as soon as its
-  // products are out, into its place) and the fetches of a later one
-  auto read_w = [&](const char* p, int a) __attribute__((always_inline)) {
-    w[a] = *(const i32x4*)(p + w_pos + 1024 * a);
-    ws[a] = *(const int*)(p + ws_pos + 16 * kScaleRow * a);
+  // one stage's operands besides the first seven row tiles of W: two sets take turns
+  struct Operands {
+    i32x8 h[kCT];
+    i32x4 w7;
+    int hs[kCT], ws7;
+  } even, odd;
+  i32x4 w[7];
+  int ws[7];
+  auto read_w = [&](const char* p, i32x4& w, int a) __attribute__((always_inline)) { w = *(const i32x4*)(p + w_pos + 1024 * a); };
+  auto read_ws = [&](const char* p, int& ws, int a) __attribute__((always_inline)) {
+    ws = *(const int*)(p + ws_pos + 16 * kScaleRow * a);
   };
-  auto read_h = [&](const char* p, i32x8(&h)[kCT], int(&hs)[kCT], int b) __attribute__((always_inline)) {
-    const i32x4 lo = *(const i32x4*)(p + h_pos0 + 2048 * b), hi = *(const i32x4*)(p + h_pos1 + 2048 * b);
-    h[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    hs[b] = *(const int*)(p + hs_pos + 16 * kScaleRow * b);
+  auto read_h = [&](const char* p, Operands& o, int i) __attribute__((always_inline)) {  // instruction i of 3 kCT
+    const int b = i / 3;
+    if (i % 3 == 0) {
+      const i32x4 lo = *(const i32x4*)(p + h_pos0 + 2048 * b);
+      o.h[b] = __builtin_shufflevector(lo, lo, 0, 1, 2, 3, -1, -1, -1, -1);
+    } else if (i % 3 == 1) {
+      const i32x4 hi = *(const i32x4*)(p + h_pos1 + 2048 * b);
+      o.h[b] = __builtin_shufflevector(o.h[b], __builtin_shufflevector(hi, hi, 0, 1, 2, 3, -1, -1, -1, -1), 0, 1, 2, 3, 8, 9, 10, 11);
+    } else {
+      o.hs[b] = *(const int*)(p + hs_pos + 16 * kScaleRow * b);
+    }
   };
-  auto stage = [&](const i32x8(&h)[kCT], const int(&hs_raw)[kCT], i32x8(&h_next)[kCT], int(&hs_next)[kCT], const char* read,
-                   char* free_place, f32x4(&acc)[8][kCT]) __attribute__((always_inline)) {
-    constexpr int kSlots = 4 * kCT;
+  // One stage: its products, and before each of them at most two of the next stage's reads (H's first, a row tile of
+  // W's as soon as its products are out, into its place) and of a later one's fetches: a product takes 32 cycles, in
+  // which what is issued behind it goes unnoticed.
+  auto stage = [&](const Operands& o, Operands& next, const char* read, char* free_place,
+                   f32x4(&acc)[8][kCT]) __attribute__((always_inline)) {
+    constexpr int kSlots = 8 * kCT;
     int hs[kCT];
 #pragma unroll
-    for (int b = 0; b < kCT; ++b) hs[b] = hs_raw[b] >> shift;
+    for (int b = 0; b < kCT; ++b) hs[b] = o.hs[b] >> shift;
 #pragma unroll
     for (int t = 0; t < kSlots; ++t) {
-      if (t % 3 == 0 && t / 3 < kCT) read_h(read, h_next, hs_next, t / 3);
-      if (t > 0 && 2 * t % kCT == 0) read_w(read, 2 * t / kCT - 1);
+      const int a = t / kCT, b = t % kCT;
+#pragma unroll
+      for (int i = (3 * t + 3) / 4; i < (3 * t + 6) / 4 && i < 3 * kCT; ++i) read_h(read, next, i);
+      if (t == kSlots / 2) read_w(read, next.w7, 7);
+      if (t == kSlots / 2 + 2) read_ws(read, next.ws7, 7);
+      if (a > 0 && b == kCT / 2 - 1) read_w(read, w[a - 1], a - 1);
+      if (a > 0 && b == kCT - 1) read_ws(read, ws[a - 1], a - 1);
 #pragma unroll
       for (int i = (t * T::kFetches + kSlots - 1) / kSlots; i < ((t + 1) * T::kFetches + kSlots - 1) / kSlots; ++i)
         fetch(i, free_place);
 #ifdef __HIP_DEVICE_COMPILE__
       __builtin_amdgcn_sched_barrier(0x6);
 #endif
-#pragma unroll
-      for (int q = 2 * t; q < 2 * t + 2; ++q)
-        add_scaled_products(acc[q / kCT][q % kCT], w[q / kCT], h[q % kCT], ws[q / kCT] >> shift, hs[q % kCT]);
+      if (a < 7) add_scaled_products(acc[a][b], w[a < 7 ? a : 0], o.h[b], ws[a < 7 ? a : 0] >> shift, hs[b]);
+      else add_scaled_products(acc[a][b], o.w7, o.h[b], o.ws7 >> shift, hs[b]);
 #ifdef __HIP_DEVICE_COMPILE__
       __builtin_amdgcn_sched_barrier(0x6);
 #endif
     }
-    read_w(read, 7);
   };
 
   fetch_tile();
@@ -509,12 +534,15 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
     fetch_next();
   }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kAhead) : "memory");
-  i32x8 h0[kCT], h1[kCT];
-  int hs0[kCT], hs1[kCT];
 #pragma unroll
-  for (int b = 0; b < kCT; ++b) read_h(lds, h0, hs0, b);
+  for (int i = 0; i < 3 * kCT; ++i) read_h(lds, even, i);
 #pragma unroll
-  for (int a = 0; a < 8; ++a) read_w(lds, a);
+  for (int a = 0; a < 7; ++a) {
+    read_w(lds, w[a], a);
+    read_ws(lds, ws[a], a);
+  }
+  read_w(lds, even.w7, 7);
+  read_ws(lds, even.ws7, 7);
   // (the first place is read by every wave before it is fetched into)
   asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
   int stored = 0;  // stages to come whose wait need not cover the stores of a tile
@@ -540,19 +568,15 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
     };
     int kb = 0;
     for (; kb + 1 < nk; kb += 2) {
-      stage(h0, hs0, h1, hs1, lds + ring[1], lds + ring[0], acc);
+      stage(even, odd, lds + ring[1], lds + ring[0], acc);
       next_stage();
-      stage(h1, hs1, h0, hs0, lds + ring[1], lds + ring[0], acc);
+      stage(odd, even, lds + ring[1], lds + ring[0], acc);
       next_stage();
     }
     if (kb < nk) {
-      stage(h0, hs0, h1, hs1, lds + ring[1], lds + ring[0], acc);
+      stage(even, odd, lds + ring[1], lds + ring[0], acc);
       next_stage();
-#pragma unroll
-      for (int b = 0; b < kCT; ++b) {
-        h0[b] = h1[b];
-        hs0[b] = hs1[b];
-      }
+      even = odd;
     }
     sums_ready();
     // lane (j, g) holds column j of H's rows, rows 4 g + e of W's
@@ -565,72 +589,75 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
     const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc(
         (void*)(out + (size_t)m0 * V + v0), (short)0, (int)(((int64_t)m_rows * V - v0) * 4), kBufferWord3);
     // The next stage's place is free until its fetches: its operands are in registers, and every wave's reads of it
-    // are done. 16-byte piece c of staged row r lies at piece c ^ (r & 15): the lanes of a write hit different banks.
-    // The softcap comes after the way through LDS, where the values are not bound to the sums' registers.
-    char* stage_out = lds + ring[0];
-    auto store_row = [&](int r, int row, const float (&x)[4]) __attribute__((always_inline)) {
+    // are done. A wave has 8 KB of it for 16 rows at a time, and waits for no other one. 16-byte piece c of staged
+    // row r lies at piece c ^ r: the lanes of a write hit different banks. The softcap comes after the way through
+    // LDS, where the values are not bound to the sums' registers.
+    char* stage_out = lds + ring[0] + 8192 * wave;
+    const int half = l >> 5, piece = l & 31, row_of = 16 * kCT * wm, v_of = 128 * wv;
+    auto store_rows = [&](int b, int i, const float (&x)[4]) __attribute__((always_inline)) {
+      const int row = row_of + 16 * b + 2 * i + half;
       if (kPieces) {
         const f32x4 y{x[0], x[1], x[2], x[3]};
+        const int v = v_of + 4 * piece;
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(MxU32x4, y), rows,
-                                               v0 + 4 * l < V ? (uint32_t)(row * V + 4 * l) * 4u : kBufferOutOfRange, 0, kOutCache);
+                                               v0 + v < V ? (uint32_t)(row * V + v) * 4u : kBufferOutOfRange, 0, kOutCache);
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
+        for (int e = 0; e < 4; ++e) {
+          const int v = v_of + 32 * e + piece;
           __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x[e]), rows,
-                                                v0 + 64 * e + l < V ? (uint32_t)(row * V + 64 * e + l) * 4u : kBufferOutOfRange, 0, kOutCache);
+                                                v0 + v < V ? (uint32_t)(row * V + v) * 4u : kBufferOutOfRange, 0, kOutCache);
+        }
       }
     };
-    auto load_row = [&](int r, float (&x)[4]) __attribute__((always_inline)) {
+    auto load_rows = [&](int i, float (&x)[4]) __attribute__((always_inline)) {
+      const int r = 2 * i + half;
       if (kPieces) {
-        const f32x4 y = *(const f32x4*)(stage_out + r * 1024 + ((l ^ (r & 15)) * 16));
+        const f32x4 y = *(const f32x4*)(stage_out + r * 512 + ((piece ^ r) * 16));
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = y[e];
       } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = 64 * e + l;
-          x[e] = *(const float*)(stage_out + r * 1024 + (((v >> 2) ^ (r & 15)) * 16) + 4 * (v & 3));
-        }
+        for (int e = 0; e < 4; ++e) x[e] = *(const float*)(stage_out + r * 512 + (((8 * e + (piece >> 2)) ^ r) * 16) + 4 * (piece & 3));
       }
     };
 #pragma unroll
     for (int b = 0; b < kCT; ++b) {
+      wave_order();
 #pragma unroll
-      for (int a = 0; a < 8; ++a)
-        *(f32x4*)(stage_out + (16 * wm + ej) * 1024 + (((32 * wv + 4 * a + eg) ^ ej) * 16)) = acc[a][b];
-      lds_barrier();
+      for (int a = 0; a < 8; ++a) *(f32x4*)(stage_out + ej * 512 + (((4 * a + eg) ^ ej) * 16)) = acc[a][b];
+      wave_order();
       float x[8][4], square[8][4], largest = 0.0f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        load_row(8 * wave + i, x[i]);
+        load_rows(i, x[i]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           square[i][e] = x[i][e] * x[i][e];
           largest = __builtin_fmaxf(largest, square[i][e]);  // (passes by NaN, which the series keeps)
         }
       }
-      auto row_of = [&](int r) { return 16 * kCT * (r >> 4) + 16 * b + (r & 15); };  // of the tile
       if (cap <= 0.0f) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) store_row(8 * wave + i, row_of(8 * wave + i), x[i]);
+        for (int i = 0; i < 8; ++i) store_rows(b, i, x[i]);
       } else if (__all(largest < reach)) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[i][e] *= series(square[i][e]);
-          store_row(8 * wave + i, row_of(8 * wave + i), x[i]);
+          store_rows(b, i, x[i]);
         }
       } else {
 #pragma unroll 1
         for (int i = 0; i < 8; ++i) {
           float y[4];
-          load_row(8 * wave + i, y);
+          load_rows(i, y);
           cap_logits(y, cap, series);
-          store_row(8 * wave + i, row_of(8 * wave + i), y);
+          store_rows(b, i, y);
         }
       }
-      lds_barrier();  // read before the next rows take the place
     }
+    lds_barrier();  // every wave has read its rows before a fetch takes the place
     stored = T::kPlaces - 2;
   }
   // no fetch is under way to LDS that the next workgroup may get
