@@ -386,10 +386,13 @@ const char* mx_error(gs_context* ctx, int32_t dtype, int32_t format, int64_t row
   return nullptr;
 }
 
+constexpr const char* kBadCap = "softcap must be finite";
+
 // The sizes of a loss call. The kernels address H, a piece of W and a piece of
 // the gradients with 31-bit byte offsets.
-int loss_check(gs_context* ctx, int32_t rows, int32_t width) {
+int loss_check(gs_context* ctx, int32_t rows, int32_t width, float softcap) {
   if (!ctx || rows < 0 || width <= 0) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "bad arguments");
+  if (!std::isfinite(softcap)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, kBadCap);
   if (width % 64 != 0 || width > 65536)
     return fail(ctx, GS_ERR_UNSUPPORTED, "lm_head width must be a multiple of 64, at most 65536");
   if (rows > kHeadMaxRows || (int64_t)rows * width >= ((int64_t)1 << 30))
@@ -1295,6 +1298,7 @@ int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hi
                  const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t m_rows, int32_t width,
                  float softcap, float* logits, void* stream) {
   if (!ctx || m_rows < 0 || width <= 0) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "bad arguments");
+  if (!std::isfinite(softcap)) return fail(ctx, GS_ERR_INVALID_ARGUMENT, kBadCap);
   if (width % 64 != 0 || width > kMxHeadMaxWidth)
     return fail(ctx, GS_ERR_UNSUPPORTED, "microscaled lm_head width must be a multiple of 64, at most 16384");
   if (m_rows > kHeadMaxRows || (int64_t)(ctx->vocab / 256 + 8) * ((m_rows + 127) / 128) > kMaxTiles)
@@ -1332,7 +1336,7 @@ int gs_mx_lmhead_sample(gs_context* ctx, const uint8_t* hidden_codes, const uint
 
 int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets, int32_t rows,
                    int32_t width, float softcap, float* loss, float* lse, void* stream) {
-  int st = loss_check(ctx, rows, width);
+  int st = loss_check(ctx, rows, width, softcap);
   if (st != GS_OK || rows == 0) return st;
   if (!hidden || !weight || !targets || !loss || !lse)
     return fail(ctx, GS_ERR_INVALID_ARGUMENT, "hidden, weight, targets, loss and lse are required");
@@ -1354,7 +1358,7 @@ int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, cons
 int gs_lmhead_loss_grad(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets,
                         const float* lse, const float* dloss, int32_t rows, int32_t width, float softcap,
                         void* dhidden, void* dweight, void* stream) {
-  int st = loss_check(ctx, rows, width);
+  int st = loss_check(ctx, rows, width, softcap);
   if (st != GS_OK) return st;
   if (rows && !dhidden && !dweight) return fail(ctx, GS_ERR_INVALID_ARGUMENT, "no output is given");
   if (!aligned16(dhidden) || !aligned16(dweight))

@@ -374,8 +374,10 @@ int gs_mx_dequantize(gs_context* ctx, const uint8_t* codes, const uint8_t* scale
 /* The lm_head over microscaled operands: logits[m][v] = cap(hidden[m] . weight[v])
  * with hidden in e4m3 ([m_rows][width], scales [m_rows][width / 32]) and weight in
  * e2m1 ([V][width / 2], scales [V][width / 32]), both as gs_mx_quantize lays them
- * out, sums in binary32, the cap as gs_lmhead's. width a multiple of 64, at most
- * 16384; codes 16-byte, scales 2-byte aligned. logits f32 [m_rows][V]. */
+ * out, the cap as gs_lmhead's (softcap finite; <= 0: none). width a multiple of 64,
+ * at most 16384; codes 16-byte, scales 2-byte aligned. logits f32 [m_rows][V].
+ * Sums are in binary32 but for the matrix instruction's own: it adds 8 neighbouring
+ * products at a time, each cut 13 bits below the largest of them. */
 int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
                  const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t m_rows, int32_t width,
                  float softcap, float* logits, void* stream);
@@ -389,8 +391,8 @@ int gs_mx_lmhead_sample(gs_context* ctx, const uint8_t* hidden_codes, const uint
  * loss[m] = lse[m] - z[m][targets[m]], 0 where the target is outside [0, V) (a
  * row that is not scored). hidden bf16 [rows][width], weight bf16 [V][width],
  * 16-byte aligned, width a multiple of 64; targets int32 [rows]; loss and lse f32
- * [rows]. width at most 65536, rows at most 2^20, rows * width below 2^30. Takes the
- * context's work memory. */
+ * [rows]. width at most 65536, rows at most 2^20, rows * width below 2^30; softcap
+ * finite (<= 0: none). Takes the context's work memory. */
 int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, const int32_t* targets, int32_t rows,
                    int32_t width, float softcap, float* loss, float* lse, void* stream);
 /* Its gradients for dloss (f32 [rows], the gradient of loss; not read where a row

@@ -260,3 +260,15 @@ def test_refusals(samplers):
     ):
         with pytest.raises(gsample.GSampleError):
             call()
+
+
+@pytest.mark.parametrize("cap", [float("nan"), float("inf"), -float("inf")])
+def test_a_cap_that_is_not_finite_is_refused(samplers, cap):
+    import gsample
+
+    h, w = torch.zeros(4, 64, dtype=torch.bfloat16).cuda(), torch.zeros(300, 64, dtype=torch.bfloat16).cuda()
+    t, f = torch.zeros(4, dtype=torch.int32).cuda(), torch.zeros(4).cuda()
+    with pytest.raises(gsample.GSampleError, match="softcap must be finite"):
+        samplers(300).lmhead_loss(h, w, t, softcap_value=cap)
+    with pytest.raises(gsample.GSampleError, match="softcap must be finite"):
+        samplers(300).lmhead_loss_grad(h, w, t, f, f, softcap_value=cap)

@@ -267,3 +267,12 @@ def test_refusals(samplers):
     ):
         with pytest.raises(gsample.GSampleError):
             call()
+
+
+@pytest.mark.parametrize("cap", [float("nan"), float("inf"), -float("inf")])
+def test_a_cap_that_is_not_finite_is_refused(samplers, cap):
+    import gsample
+
+    z = lambda *shape: torch.zeros(*shape, dtype=torch.uint8).cuda()  # noqa: E731
+    with pytest.raises(gsample.GSampleError, match="softcap must be finite"):
+        samplers(512).mx_lmhead(z(3, 64), z(3, 2), z(512, 32), z(512, 2), softcap_value=cap)
