@@ -584,8 +584,9 @@ class Sampler:
     # -- the operators on either side of the head ------------------------
     # Each takes the memory of its results (allocated when left out) and a
     # stream. With a stream it enqueues there and returns; inputs must be ready
-    # on that stream. Without one it waits for torch's current stream, runs on
-    # the context's and waits for the results.
+    # on that stream. Without one, or with 0 (the handle of torch's default
+    # stream, which the library reads as the context's own), it waits for torch's
+    # current stream, runs on the context's and waits for the results.
     def _tensor(self, t, name: str, dtype, shape=None):
         """The pointer of a checked contiguous tensor (None: NULL)."""
         if t is None:
@@ -624,17 +625,17 @@ class Sampler:
         """Memory for a result of a call on `stream`: the caching allocator must
         not hand it out again before that stream has used it."""
         t = self.torch.empty(shape, dtype=dtype, device=self.device)
-        if stream is not None and self.torch.cuda.current_stream(self.device).cuda_stream != stream:
+        if stream and self.torch.cuda.current_stream(self.device).cuda_stream != stream:
             t.record_stream(self.torch.cuda.ExternalStream(stream, device=self.device))
         return t
 
     def _begin(self, stream):
-        if stream is None:
+        if not stream:
             self.torch.cuda.current_stream(self.device).synchronize()
         return stream or None
 
     def _end(self, stream):
-        if stream is None:
+        if not stream:
             self.synchronize()
 
     def rms_norm(self, x, weight, residual=None, eps: float = 1e-6, weight_offset: float = 0.0, out=None, summed=None,

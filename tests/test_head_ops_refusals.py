@@ -66,6 +66,21 @@ def test_refused_before_the_library(sampler, call, message):
     assert e.value.status == 1
 
 
+@pytest.mark.parametrize("stream,waits", [(None, 1), (0, 1), (77, 0)])
+def test_the_default_stream_is_waited_for(sampler, stream, waits):
+    """0, the default stream's handle, stands for the context's own stream in the library."""
+    from types import SimpleNamespace
+
+    seen = []
+    current = SimpleNamespace(synchronize=lambda: seen.append("inputs"), cuda_stream=77)
+    sampler.torch = SimpleNamespace(cuda=SimpleNamespace(current_stream=lambda device: current), empty=torch.empty)
+    sampler.synchronize = lambda: seen.append("results")
+    assert sampler._begin(stream) == (stream or None)
+    assert sampler._empty((2,), torch.float32, stream).shape == (2,)
+    sampler._end(stream)
+    assert seen == ["inputs", "results"][:2 * waits]
+
+
 def test_other_devices_are_refused(sampler):
     sampler.device = torch.device("cuda", 0)
     with pytest.raises(gsample.GSampleError, match="sampler's device"):
