@@ -197,6 +197,11 @@ int ensure_work(gs_context* ctx, size_t bytes, hipStream_t s) {
   if (capture != hipStreamCaptureStatusNone)
     return fail(ctx, GS_ERR_UNSUPPORTED, "the work memory cannot grow under capture: make the call once before it");
   const size_t want = ctx->work_cap ? bytes + bytes / 4 : bytes;
+  try {  // (nothing is thrown through the C entry, and no block is lost)
+    ctx->old_work.reserve(ctx->old_work.size() + 1);
+  } catch (const std::exception&) {
+    return fail(ctx, GS_ERR_HIP, "out of host memory");
+  }
   uint8_t* p = nullptr;
   if (hipMalloc(&p, want) != hipSuccess) {
     (void)hipGetLastError();
