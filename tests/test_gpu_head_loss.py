@@ -86,6 +86,10 @@ def test_a_large_vocabulary_in_pieces(samplers):
     check(samplers(vocab), h, w, t, 30.0)
 
 
+def test_the_largest_vocabulary(samplers):
+    check(samplers(2097152), *operands(np.random.default_rng(27), 3, 64, 2097152, 2.0), 30.0)
+
+
 def test_confident_rows_and_far_logits(samplers):
     """Targets whose probability is near one, and logits of +-100 without a cap."""
     rng = np.random.default_rng(22)

@@ -191,6 +191,22 @@ def test_head_of_many_tiles(samplers, m, width, vocab, cap, shift):
             assert ((out[r:r + n] - few).abs() <= 1e-3 * (1 + few.abs())).all()
 
 
+@pytest.mark.parametrize("m", [3, 100, 256])
+def test_head_of_the_largest_vocabulary(samplers, m):
+    """Tiles of the logits whose byte offsets reach 2^31 (256 rows)."""
+    vocab, width = 2097152, 64
+    gen = torch.Generator(device="cuda:0").manual_seed(m)
+    code = lambda *shape, lo=0, hi=256: torch.randint(lo, hi, shape, dtype=torch.uint8, device="cuda:0", generator=gen)  # noqa: E731
+    hc, hs, wc, ws = code(m, width, hi=0x7f), code(m, 2, lo=124, hi=130), code(vocab, width // 2), code(vocab, 2, lo=118, hi=128)
+    out = samplers(vocab).mx_lmhead(hc, hs, wc, ws, softcap_value=0.0)
+    some = np.unique(np.concatenate([np.random.default_rng(m).integers(0, vocab, 400), np.arange(260), np.arange(vocab - 260, vocab)]))
+    at = torch.from_numpy(some).cuda()
+    w = wc[at].cpu().numpy()
+    wv = ref.mx_dequantize(np.stack([w & 15, w >> 4], -1).reshape(len(some), width), ws[at].cpu().numpy(), "e2m1")
+    hv = ref.mx_dequantize(hc.cpu().numpy(), hs.cpu().numpy(), "e4m3")
+    check_logits(out[:, at], torch.from_numpy(hv), torch.from_numpy(wv), 0.0)
+
+
 def test_a_special_block_stays_in_its_own_logit(samplers):
     rng = np.random.default_rng(12)
     for width in (64, 320, 512):
