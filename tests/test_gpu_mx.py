@@ -82,6 +82,29 @@ def test_every_code_reads_back(samplers):
             assert np.array_equal(got, want.astype(np.float32), equal_nan=True)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+def test_many_blocks_read_back_as_in_slices(samplers, fmt, dtype):
+    gen = torch.Generator(device="cuda:0").manual_seed(3)
+    rows, width = 349526, 96  # over 2^22 groups of 8, and no multiple of a workgroup's
+    x = torch.randn(rows, width, device="cuda:0", generator=gen)
+    s = samplers(1000)
+    codes, scales = s.mx_quantize(x, fmt)
+    whole = torch.full((rows + 1, width), 7.0, dtype=dtype).cuda()
+    s.mx_dequantize(codes, scales, fmt, out=whole[:rows])
+    for a, b in ((0, 100), (100, 4000), (rows - 3000, rows)):
+        some = s.mx_quantize(x[a:b], fmt)
+        assert torch.equal(some[0], codes[a:b]) and torch.equal(some[1], scales[a:b])
+        assert torch.equal(s.mx_dequantize(*some, fmt, dtype=dtype), whole[a:b])
+    # The scale puts a block's largest magnitude m at 4 to 8 (e2m1) or 256 to 512 (e4m3). Past 6 or 448 it becomes
+    # that: off by less than m - 6 <= m 2/8, or m - 448 <= m 64/512. Anything else is off by at most half a step of the
+    # top binade, 1 <= m/4, or 16 <= m/16. bf16 holds every one of these values (and the subtraction below rounds).
+    off = (whole[:rows].float() - x).abs().view(rows, -1, 32)
+    most = x.abs().view(rows, -1, 32).amax(2) * (2.0 ** -2 if fmt == "e2m1" else 2.0 ** -3) * (1 + 2.0 ** -20)
+    assert (off.amax(2) <= most).all()
+    assert (whole[rows] == 7.0).all()
+
+
 def test_strided_rows_and_no_rows(samplers):
     s = samplers(512)
     rng = np.random.default_rng(3)
