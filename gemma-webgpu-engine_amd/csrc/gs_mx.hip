@@ -97,9 +97,11 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t
 //
 // ---- up to 64 hidden rows: bound by W's bytes
 // Tiles of 256 vocabulary rows by kCols hidden rows, 8 waves, 256 columns of K a
-// stage, three stages in LDS, two of them on the way. 1 row by 262144 x 1536: 42 us
-// for 214 MB, 5.1 TB/s; 64 rows by 262144 x 2048: 74 us for 352 MB (67 MB of them
-// logits), 4.8 TB/s; a copy reaches 5.2.
+// stage, three stages in LDS, two of them on the way. A workgroup a compute unit
+// takes tile after tile, so that the next tile's data come while the logits go out
+// (a workgroup a tile: 3 us more). 1 row by 262144 x 1536: the kernel 34 us for 214
+// MB, 6.3 TB/s; 64 rows by 262144 x 2048: 70 us for 352 MB (67 MB of them logits),
+// 5.0 TB/s; a copy reaches 5.2.
 //
 // K order: the instruction multiplies four blocks of 32 at a time, one a group
 // of 16 lanes. Step s (of two) of a stage takes blocks s, 2 + s, 4 + s, 6 + s,
@@ -111,6 +113,7 @@ constexpr int kHeadThreads = 512;
 constexpr int kHeadRows = 256;   // vocabulary rows a tile
 constexpr int kHeadK = 256;      // columns a stage
 constexpr int kHeadStride = kHeadRows + 4;  // LDS floats per staged output row
+constexpr int kOutCache = 2;  // non-temporal: the logits are streamed once
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -128,7 +131,10 @@ struct HeadTile {
   static constexpr int kHS = kCols * 16;              // of H
   static constexpr int kStage = kW + kH + kWS + kHS;
   static constexpr int kFetches = 4 + kCols / 32 + 3; // memory instructions of a wave and stage
+  static constexpr int kAhead = (kStages - 2) * kFetches;  // newer than the stage that has to have landed
+  static constexpr int kPieceStores = kCols / 8;           // 16-byte stores of a wave and tile
   static constexpr int kHeadLds = kStages * kStage + 256;  // and where waves without scales of H put theirs
+  static_assert(kHeadLds <= 160 * 1024 && 32 * kHeadStride * 4 <= kStage, "LDS of a compute unit");
 };
 
 struct HeadOffsets {
@@ -161,14 +167,11 @@ __device__ __forceinline__ void head_fetch(char* lds, char* spare, int wave, Rsr
 #endif
 }
 
-// One stage: the next fetches go out, then two steps of 128 columns.
-template <int kCols, typename Rsrc>
-__device__ __forceinline__ void head_block(const char* __restrict__ cur, char* __restrict__ next, char* spare, int wave,
-                                           int wv, int j, int g, Rsrc wr, Rsrc hr, Rsrc wsr, Rsrc hsr,
-                                           const HeadOffsets& o, uint32_t k, bool tail, bool none,
+// One stage's products, two steps of 128 columns.
+template <int kCols>
+__device__ __forceinline__ void head_block(const char* __restrict__ cur, int wv, int j, int g,
                                            f32x4 (&acc)[HeadTile<kCols>::kRT][HeadTile<kCols>::kCT]) {
   typedef HeadTile<kCols> T;
-  head_fetch<kCols>(next, spare, wave, wr, hr, wsr, hsr, o, k, tail, none);
   const char* w = cur + (16 * T::kRT * wv + j) * 128;
   const char* h = cur + T::kW + j * 256;
   const int* ws = (const int*)(cur + T::kW + T::kH) + (16 * T::kRT * wv + j) * 4 + g;
@@ -203,32 +206,35 @@ __device__ __forceinline__ void head_block(const char* __restrict__ cur, char* _
   }
 }
 
-template <int kCols>
+// Waits until at most kAhead memory instructions are under way (kAheadStores
+// where a tile's stores are among them), and for every wave. The choice is in the
+// assembly: around it, it would double the stage.
+template <int kAhead, int kAheadStores>
+__device__ __forceinline__ void landed(int stored) {
+  asm volatile(
+      "s_cmp_lg_u32 %0, 0\n\t"
+      "s_cbranch_scc1 .Llanded%=\n\t"
+      "s_waitcnt vmcnt(%1)\n\t"
+      ".Llanded%=:\n\t"
+      "s_waitcnt vmcnt(%2) lgkmcnt(0)\n\t"
+      "s_barrier" ::"s"(stored),
+      "n"(kAhead), "n"(kAheadStores)
+      : "memory", "scc");
+}
+
+// kPieces: 16-byte pieces of a logits row (V % 4 == 0 and aligned logits).
+template <int kCols, bool kPieces>
 __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
     const uint8_t* __restrict__ H, const uint8_t* __restrict__ HS, const uint8_t* __restrict__ W,
-    const uint8_t* __restrict__ WS, int M, int D, int V, int m_blocks, int wide, float cap, float* __restrict__ out) {
+    const uint8_t* __restrict__ WS, int M, int D, int V, int tiles, float cap, float* __restrict__ out) {
   typedef HeadTile<kCols> T;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  // consecutive workgroups go to the XCDs in turn: an XCD takes the row
-  // blocks of one tile of W one after another
-  const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-  const int vt = (local / m_blocks) * 8 + xcd;
-  const int64_t v0 = (int64_t)vt * kHeadRows, m0 = (int64_t)(local % m_blocks) * kCols;
-  if (v0 >= V) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int j = lane & 15, g = lane >> 4, wv = wave;
-  const int v_rows = V - v0 < kHeadRows ? (int)(V - v0) : kHeadRows;
-  const int m_rows = M - m0 < kCols ? (int)(M - m0) : kCols;
+  const int j = lane & 15, g = lane >> 4;
   const int ds = D / 32;
   // rows past V or M read zeros (and scales of 2^-127)
-  const __amdgpu_buffer_rsrc_t wr =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(W + (size_t)v0 * (D / 2)), (short)0, v_rows * (D / 2), kBufferWord3);
-  const __amdgpu_buffer_rsrc_t hr =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(H + (size_t)m0 * D), (short)0, m_rows * D, kBufferWord3);
-  const __amdgpu_buffer_rsrc_t wsr =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(WS + (size_t)v0 * ds), (short)0, v_rows * ds, kBufferWord3);
-  const __amdgpu_buffer_rsrc_t hsr =
-      __builtin_amdgcn_make_buffer_rsrc((void*)(HS + (size_t)m0 * ds), (short)0, m_rows * ds, kBufferWord3);
+  const __amdgpu_buffer_rsrc_t hr = __builtin_amdgcn_make_buffer_rsrc((void*)H, (short)0, M * D, kBufferWord3);
+  const __amdgpu_buffer_rsrc_t hsr = __builtin_amdgcn_make_buffer_rsrc((void*)HS, (short)0, M * ds, kBufferWord3);
   // Fetched rows: 16-byte chunk c of row r lands at chunk c ^ (r & 7), so that
   // the lanes of an operand read that go together hit different banks.
   HeadOffsets o;
@@ -250,66 +256,95 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
   o.hs = 16 * wave < kCols ? (uint32_t)((16 * wave + (lane >> 2)) * ds + 2 * (lane & 3)) : kBufferOutOfRange;
   o.s_tail = 64 * (lane & 3) < last_k ? 0u : kBufferOutOfRange;
 
-  f32x4 acc[T::kRT][T::kCT];
-#pragma unroll
-  for (int a = 0; a < T::kRT; ++a) {
-#pragma unroll
-    for (int b = 0; b < T::kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
+  // what is fetched next: tiles start at different columns, so that their reads spread over the memory channels
   char* spare = lds + T::kStages * T::kStage;
-  // tiles start at different columns: their reads spread over the memory channels
-  const int first = vt % nk;
-  auto at = [&](int kb) __attribute__((always_inline)) {
-    const int k = (kb < nk ? kb : 0) + first;
-    return k < nk ? k : k - nk;
+  __amdgpu_buffer_rsrc_t wr, wsr;
+  int f_id = (int)blockIdx.x, f_left = 0, f_k = 0;
+  auto fetch_tile = [&]() __attribute__((always_inline)) {
+    const int v0 = f_id < tiles ? f_id * kHeadRows : 0;
+    const int v_rows = f_id < tiles ? (V - v0 < kHeadRows ? V - v0 : kHeadRows) : 0;  // (past the last tile: nothing)
+    wr = __builtin_amdgcn_make_buffer_rsrc((void*)(W + (size_t)v0 * (D / 2)), (short)0, v_rows * (D / 2), kBufferWord3);
+    wsr = __builtin_amdgcn_make_buffer_rsrc((void*)(WS + (size_t)v0 * ds), (short)0, v_rows * ds, kBufferWord3);
+    f_left = nk;
+    f_k = f_id % nk;
   };
-  auto partial = [&](int k) __attribute__((always_inline)) { return k == nk - 1 && last_k < kHeadK; };
-#pragma unroll
-  for (int u = 0; u < T::kStages - 1; ++u)
-    head_fetch<kCols>(lds + u * T::kStage, spare, wave, wr, hr, wsr, hsr, o, (uint32_t)at(u), partial(at(u)), u >= nk);
-  for (int kb = 0; kb < nk; kb += T::kStages) {
-#pragma unroll
-    for (int u = 0; u < T::kStages; ++u) {
-      if (kb + u < nk) {
-        // the stage has landed for every wave, and every wave has read the one before
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((T::kStages - 2) * T::kFetches) : "memory");
-        const int n = kb + u + T::kStages - 1, k = at(n);
-        head_block<kCols>(lds + u * T::kStage, lds + (u + T::kStages - 1) % T::kStages * T::kStage, spare, wave, wv, j,
-                          g, wr, hr, wsr, hsr, o, (uint32_t)k, partial(k), n >= nk, acc);
-      }
+  auto fetch = [&](char* place) __attribute__((always_inline)) {
+    head_fetch<kCols>(place, spare, wave, wr, hr, wsr, hsr, o, (uint32_t)f_k, f_k == nk - 1 && last_k < kHeadK, f_id >= tiles);
+    if (--f_left == 0) {
+      f_id = f_id < tiles ? f_id + (int)gridDim.x : f_id;
+      fetch_tile();
+    } else {
+      f_k = f_k + 1 < nk ? f_k + 1 : 0;
     }
-  }
-  // nothing is in flight to or from LDS before the outputs take its place
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-
-  // the cap, then the tile through LDS, so that rows go out in pieces of 1 KB
-  // (lane (j, g) holds column j of H's rows, rows 4 g + e of W's)
-  float* stage = (float*)lds;
-  const CapSeries series(cap, 1.0f);
+  };
+  fetch_tile();
+  int ring[T::kStages];
 #pragma unroll
-  for (int b = 0; b < T::kCT; ++b) {
+  for (int u = 0; u < T::kStages; ++u) {
+    ring[u] = u * T::kStage;
+    if (u < T::kStages - 1) fetch(lds + ring[u]);
+  }
+  int stored = 0;  // stages to come whose wait need not cover the stores of a tile
+  const CapSeries series(cap, 1.0f);
+  for (int id = (int)blockIdx.x; id < tiles; id += (int)gridDim.x) {
+    f32x4 acc[T::kRT][T::kCT];
 #pragma unroll
     for (int a = 0; a < T::kRT; ++a) {
-      float x[4] = {acc[a][b][0], acc[a][b][1], acc[a][b][2], acc[a][b][3]};
-      if (cap > 0.0f) cap_logits(x, cap, series);
-      *(f32x4*)&stage[(16 * b + j) * kHeadStride + 16 * (T::kRT * wv + a) + 4 * g] =
-          f32x4{x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int b = 0; b < T::kCT; ++b) acc[a][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    for (int kb = 0; kb < nk; ++kb) {
+      // the stage has landed for every wave, and every wave has read the one before
+      landed<T::kAhead, T::kAhead + (kPieces ? 1 : 4) * T::kPieceStores>(stored);
+      asm volatile("s_sub_u32 %0, %0, 1\n\ts_cselect_b32 %0, 0, %0" : "+s"(stored)::"scc");  // (down to 0)
+      fetch(lds + ring[T::kStages - 1]);
+      head_block<kCols>(lds + ring[0], wave, j, g, acc);
+      const int r = ring[0];
+#pragma unroll
+      for (int u = 0; u + 1 < T::kStages; ++u) ring[u] = ring[u + 1];
+      ring[T::kStages - 1] = r;
+    }
+    // The cap, then the tile through the place that was read last, 32 hidden rows at a time, so that rows go out in
+    // pieces of 1 KB (lane (j, g) holds column j of H's rows, rows 4 g + e of W's).
+    const int v0 = id * kHeadRows;
+    const __amdgpu_buffer_rsrc_t rows = __builtin_amdgcn_make_buffer_rsrc((void*)(out + v0), (short)0,
+                                                                          (int)(((int64_t)M * V - v0) * 4), kBufferWord3);
+    float* stage = (float*)(lds + ring[T::kStages - 1]);
+#pragma unroll
+    for (int half = 0; half < T::kCT / 2; ++half) {
+      lds_barrier();
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+#pragma unroll
+        for (int a = 0; a < T::kRT; ++a) {
+          const f32x4 v = acc[a][2 * half + b];
+          float x[4] = {v[0], v[1], v[2], v[3]};
+          if (cap > 0.0f) cap_logits(x, cap, series);
+          *(f32x4*)&stage[(16 * b + j) * kHeadStride + 16 * (T::kRT * wave + a) + 4 * g] = f32x4{x[0], x[1], x[2], x[3]};
+        }
+      }
+      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // a wave a row at a time
+        const int r = 8 * i + wave, row = 32 * half + r;
+        if (kPieces) {
+          const f32x4 x = *(const f32x4*)&stage[r * kHeadStride + 4 * lane];
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(MxU32x4, x), rows,
+                                                 row < M && v0 + 4 * lane < V ? (uint32_t)(row * V + 4 * lane) * 4u : kBufferOutOfRange,
+                                                 0, kOutCache);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            __builtin_amdgcn_raw_buffer_store_b32(
+                __builtin_bit_cast(uint32_t, stage[r * kHeadStride + 64 * e + lane]), rows,
+                row < M && v0 + 64 * e + lane < V ? (uint32_t)(row * V + 64 * e + lane) * 4u : kBufferOutOfRange, 0, kOutCache);
+        }
+      }
+    }
+    stored = T::kStages - 1;
   }
-  __syncthreads();
-  float* p = out + (size_t)m0 * V + v0;
-  if (wide) {  // V % 4 == 0 and 16-byte aligned logits: a piece lies within its row
-    for (int q = tid; q < m_rows * (kHeadRows / 4); q += kHeadThreads) {
-      const int row = q / (kHeadRows / 4), c = 4 * (q % (kHeadRows / 4));
-      if (c < v_rows)
-        __builtin_nontemporal_store(*(const f32x4*)&stage[row * kHeadStride + c], (f32x4*)&p[(size_t)row * V + c]);
-    }
-  } else {
-    for (int q = tid; q < m_rows * kHeadRows; q += kHeadThreads) {
-      const int row = q / kHeadRows, c = q % kHeadRows;
-      if (c < v_rows) __builtin_nontemporal_store(stage[row * kHeadStride + c], &p[(size_t)row * V + c]);
-    }
-  }
+  // no fetch is under way to LDS that the next workgroup may get
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // ---- many hidden rows: bound by the matrix cores and the logits' stores
@@ -326,7 +361,6 @@ __global__ __launch_bounds__(kHeadThreads, 2) void mx_head_kernel(
 // before the way through LDS: 520 us (its far branch makes the compiler spill).
 constexpr int kWideThreads = 256;
 constexpr int kWideK = 128;
-constexpr int kOutCache = 2;  // non-temporal: the logits are streamed once
 
 // kQuads: a row's four scales of a stage are one dword (widths that are a
 // multiple of 128), else two pairs, a dword each.
@@ -362,22 +396,6 @@ __device__ __forceinline__ void sums_ready() {
   asm volatile("s_nop 15\n\ts_nop 15\n\ts_nop 15" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 #endif
-}
-
-// Waits until at most kAhead memory instructions are under way (kAheadStores
-// where a tile's stores are among them), and for every wave. The choice is in the
-// assembly: around it, it would double the stage.
-template <int kAhead, int kAheadStores>
-__device__ __forceinline__ void wide_landed(int stored) {
-  asm volatile(
-      "s_cmp_lg_u32 %0, 0\n\t"
-      "s_cbranch_scc1 .Lwide%=\n\t"
-      "s_waitcnt vmcnt(%1)\n\t"
-      ".Lwide%=:\n\t"
-      "s_waitcnt vmcnt(%2) lgkmcnt(0)\n\t"
-      "s_barrier" ::"s"(stored),
-      "n"(kAhead), "n"(kAheadStores)
-      : "memory", "scc");
 }
 
 // LDS accesses of a wave on both sides stay on their sides (it runs them in order).
@@ -577,7 +595,7 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
     auto next_stage = [&]() __attribute__((always_inline)) {
       // the stage after the next has landed for every wave, and every wave has read the next one
       constexpr int kStores = kPieces ? 8 * kCT : 32 * kCT, kBoth = T::kAhead + kStores;
-      wide_landed<T::kAhead, kBoth < 63 ? kBoth : 63>(stored);
+      landed<T::kAhead, kBoth < 63 ? kBoth : 63>(stored);
       fetch_next();
       const int r = ring[0];
 #pragma unroll
@@ -703,16 +721,16 @@ void wide_launch(const uint8_t* H, const uint8_t* HS, const uint8_t* W, const ui
 
 template <int kCols>
 void head_launch(const uint8_t* H, const uint8_t* HS, const uint8_t* W, const uint8_t* WS, int32_t m, int32_t width,
-                 int32_t vocab, float cap, float* out, hipStream_t s, LaunchEvents ev) {
+                 int32_t vocab, float cap, float* out, int32_t cu_count, hipStream_t s, LaunchEvents ev) {
   typedef HeadTile<kCols> T;
-  constexpr int kOut = kCols * kHeadStride * 4;
-  constexpr int kBytes = T::kHeadLds > kOut ? T::kHeadLds : kOut;
-  static_assert(kBytes <= 160 * 1024, "LDS of a compute unit");
-  const int m_blocks = (m + kCols - 1) / kCols, v_tiles = (vocab + kHeadRows - 1) / kHeadRows;
-  const dim3 grid((unsigned)((v_tiles + 7) / 8 * 8 * m_blocks)), block(kHeadThreads);
-  const int wide = vocab % 4 == 0 && ((uintptr_t)out & 15) == 0;
-  hipExtLaunchKernelGGL((mx_head_kernel<kCols>), grid, block, kBytes, s, ev.start, ev.stop, 0, H, HS, W, WS, m, width,
-                        vocab, m_blocks, wide, cap, out);
+  const int tiles = (vocab + kHeadRows - 1) / kHeadRows;
+  const dim3 grid((unsigned)std::min(tiles, cu_count > 0 ? cu_count : 256)), block(kHeadThreads);
+  if (vocab % 4 == 0 && ((uintptr_t)out & 15) == 0)
+    hipExtLaunchKernelGGL((mx_head_kernel<kCols, true>), grid, block, T::kHeadLds, s, ev.start, ev.stop, 0, H, HS, W, WS,
+                          m, width, vocab, tiles, cap, out);
+  else
+    hipExtLaunchKernelGGL((mx_head_kernel<kCols, false>), grid, block, T::kHeadLds, s, ev.start, ev.stop, 0, H, HS, W, WS,
+                          m, width, vocab, tiles, cap, out);
 }
 
 }  // namespace
@@ -763,8 +781,8 @@ bool wide_narrow(int32_t m, int32_t vocab, int32_t cu_count) {
 void launch_mx_lmhead(const uint8_t* hidden, const uint8_t* hidden_scales, const uint8_t* weight,
                       const uint8_t* weight_scales, int32_t m, int32_t width, int32_t vocab, float softcap, float* out,
                       int32_t cu_count, hipStream_t s, LaunchEvents ev) {
-  if (m <= 32) head_launch<32>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, s, ev);
-  else if (m <= 64) head_launch<64>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, s, ev);
+  if (m <= 32) head_launch<32>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
+  else if (m <= 64) head_launch<64>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
   else if (wide_narrow(m, vocab, cu_count))
     wide_launch<128>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
   else wide_launch<256>(hidden, hidden_scales, weight, weight_scales, m, width, vocab, softcap, out, cu_count, s, ev);
