@@ -662,6 +662,8 @@ struct LossPlan {
   int32_t cols;        // rows of H in a tile: 64, 128, 160, 192 or 256
   int32_t cus;         // compute units
   int32_t v_tiles;     // tiles of 256 vocabulary rows
+  int32_t stat_rows;   // forward: vocabulary rows of a tile, a multiple of 16, at most 256
+  int32_t stat_tiles;  // forward: tiles of as many
   int32_t piece;       // vocabulary rows whose gradients are held at a time, a multiple of 256
   int32_t splits;      // shares of a piece's vocabulary in dhidden's product
   size_t stats_bytes;  // forward: a (max, sum) per row and tile

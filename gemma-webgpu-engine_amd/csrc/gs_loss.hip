@@ -41,6 +41,7 @@ enum Pass { kStats, kGrad, kHidden, kWeight };
 constexpr int kLossThreads = 256;
 constexpr int kRows = 256;  // rows of a tile (vocabulary rows; columns of K in kHidden and kWeight)
 constexpr int kBlock = 64;  // of the summed index a stage
+constexpr int kFewRows = 128;  // columns of a tile up to which the forward pass waits for W's bytes
 constexpr float kLowest = -1.0e38f;  // a maximum over nothing; times log2(e) still finite
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -64,7 +65,8 @@ struct LossArgs {
   uint16_t* G;            // [M][g_stride]
   const Column* columns;  // [M]
   const float* most;      // the largest |dloss| of the scored rows
-  float2* stats;          // kStats: [v_tiles][M]
+  float2* stats;          // kStats: [row_tiles][M]
+  int tile_rows;          // kStats: rows of W a tile
   float* part;            // kHidden: [splits][M][D]
   uint16_t* dW;           // kWeight: the piece's first row
   float cap;
@@ -273,7 +275,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
       split = q / p.col_tiles;
       ct = q - split * p.col_tiles;
     }
-    return Place{rt * kRows, ct * kCols, split};
+    return Place{rt * (kPass == kStats ? p.tile_rows : kRows), ct * kCols, split};
   };
   auto sums_of_split = [&](int split) __attribute__((always_inline)) {
     if (kPass != kHidden) return kPass == kWeight ? M : D;
@@ -326,7 +328,8 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
       if (kPass == kStats || kPass == kGrad) {
         A = p.W + (size_t)q.r0 * D;
         B = p.H + (size_t)q.c0 * D;
-        a_bytes = (V - q.r0 < kRows ? V - q.r0 : kRows) * D * 2;
+        const int most = kPass == kStats ? p.tile_rows : kRows;
+        a_bytes = (V - q.r0 < most ? V - q.r0 : most) * D * 2;
         b_bytes = (M - q.c0 < kCols ? M - q.c0 : kCols) * D * 2;
       } else if (f_sums > 0) {
         const int sum0 = kPass == kHidden ? q.split * p.split_rows : 0;
@@ -464,24 +467,29 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
     const int ej = l & 15, eg = l >> 4;
     const int row0 = 128 * wr + 4 * eg, col0 = 16 * kCT * wc + ej;
     const int row8 = 128 * wr + 16 * (eg & 1) + 4 * (eg & 2);  // after an exchange: 8 rows from 16 a + this on, a even
-    const bool tail = V - r0 < kRows;  // (uniform; kStats, kGrad) the tile ends past the vocabulary
+    const bool tail = V - r0 < kRows;  // (uniform; kGrad) the tile ends past the vocabulary
     if constexpr (kPass == kStats) {
+      // the wave's rows, counted from row0: those past them count nothing; whole blocks of 16 are left out where
+      // tiles may be smaller (elsewhere the branches cost more, 4 % of 300 or 2048 rows)
+      const int rows = (V - r0 < p.tile_rows ? V - r0 : p.tile_rows) - 128 * wr;
+      constexpr bool kSkip = kCols <= kFewRows;
       const CapSeries series(p.cap, kLog2e);
       float2* sums_of = (float2*)scratch;  // [2][kCols]
 #pragma unroll
       for (int b = 0; b < kCT; ++b) {
         order();
-        if (tail) {  // rows past the vocabulary count nothing
+        if (kSkip ? (rows & 15) != 0 : tail) {  // (the vocabulary's last tile)
 #pragma unroll
           for (int a = 0; a < 8; ++a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (r0 + row0 + 16 * a + e >= V) acc[a][b][e] = -__builtin_inff();
+              if (16 * a + 4 * eg + e >= rows) acc[a][b][e] = -__builtin_inff();
           }
         }
         float lo = __builtin_inff(), mx = -__builtin_inff(), sum = 0.0f;
 #pragma unroll
         for (int a = 0; a < 8; ++a) {
+          if (kSkip && 16 * a >= rows) continue;  // (uniform, here and below)
           const f32x4 x = acc[a][b];
           mx = __builtin_fmaxf(__builtin_fmaxf(mx, x[0]), x[1]);
           mx = __builtin_fmaxf(__builtin_fmaxf(mx, x[2]), x[3]);
@@ -495,6 +503,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
           const float ml = -mx * kLog2e;
 #pragma unroll
           for (int a = 0; a < 8; ++a) {
+            if (kSkip && 16 * a >= rows) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[a][b][e], kLog2e, ml));
           }
@@ -505,6 +514,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
           if (__all(near)) {
 #pragma unroll
             for (int a = 0; a < 8; ++a) {
+              if (kSkip && 16 * a >= rows) continue;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float x = acc[a][b][e];
@@ -514,10 +524,11 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
           } else {
 #pragma unroll
             for (int a = 0; a < 8; ++a) {
+              if (kSkip && 16 * a >= rows) continue;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(p.cap * cap_any(acc[a][b][e] / p.cap), kLog2e, ml));
-                sum += tail && r0 + row0 + 16 * a + e >= V ? 0.0f : v;
+                sum += (kSkip || tail) && 16 * a + 4 * eg + e >= rows ? 0.0f : v;
               }
             }
           }
@@ -532,7 +543,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
         float2 s = sums_of[tid];
         const float2 o = sums_of[kCols + tid];
         join_sums(s.x, s.y, o.x, o.y);
-        p.stats[(size_t)(r0 / kRows) * M + c0 + tid] = s;
+        p.stats[(size_t)(r0 / p.tile_rows) * M + c0 + tid] = s;
       }
       lds_barrier();  // read before a fetch takes the place
     } else if constexpr (kPass == kGrad) {
@@ -817,6 +828,17 @@ LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count)
       q.cols = c;
     }
   }
+  // The forward pass of few rows waits for W's bytes, and its last round of tiles is
+  // as long as the others: tiles as small as the same number of rounds takes (a call
+  // at 100 x 2048 x 151643 128 us, 139 with tiles of 256; at 128 x 1536 x 200000 141
+  // and 153). Not within one round (17 x 704 x 32768: 21.9 us, and 20.6 with 256).
+  q.stat_rows = kRows;
+  const int64_t col_tiles = (rows + q.cols - 1) / q.cols, rounds = (q.v_tiles * col_tiles + cus - 1) / cus;
+  if (q.cols <= kFewRows && rounds > 1) {
+    const int64_t places = rounds * cus / col_tiles;  // at least v_tiles
+    q.stat_rows = (int32_t)(((vocab + places - 1) / places + 15) / 16 * 16);
+  }
+  q.stat_tiles = (vocab + q.stat_rows - 1) / q.stat_rows;
   // a piece: at most 256 MB of g, and its offsets (and W's) within 31 bits
   int64_t piece = ((int64_t)256 << 20) / ((int64_t)rows * 2);
   piece = std::min<int64_t>(piece, ((int64_t)1 << 30) / width - 256);
@@ -824,7 +846,7 @@ LossPlan loss_plan(int32_t rows, int32_t width, int32_t vocab, int32_t cu_count)
   q.piece = (int32_t)std::min<int64_t>(piece, (int64_t)q.v_tiles * 256);
   const int tiles = (width + kRows - 1) / kRows * ((rows + q.cols - 1) / q.cols);
   q.splits = std::max(1, std::min(cus / tiles, q.piece / 256));
-  q.stats_bytes = up256((size_t)q.v_tiles * rows * sizeof(float2));
+  q.stats_bytes = up256((size_t)q.stat_tiles * rows * sizeof(float2));
   q.g_bytes = up256((size_t)rows * q.piece * 2);
   q.h_bytes = up256((size_t)rows * width * 2);
   q.part_bytes = up256((size_t)q.splits * rows * width * 4);
@@ -842,12 +864,13 @@ void launch_lmhead_loss(const uint16_t* hidden, const uint16_t* weight, const in
   p.M = rows;
   p.D = width;
   p.V = vocab;
-  p.row_tiles = plan.v_tiles;
+  p.tile_rows = plan.stat_rows;
+  p.row_tiles = plan.stat_tiles;
   p.col_tiles = (rows + plan.cols - 1) / plan.cols;
   p.splits = 1;
   loss_launch<kStats>(p, plan.cols, plan.cus, s);
   loss_join_kernel<<<dim3((unsigned)((rows + kJoinRows - 1) / kJoinRows)), dim3(kJoinThreads), 0, s>>>(
-      p.stats, plan.v_tiles, hidden, weight, targets, rows, width, vocab, softcap, loss, lse);
+      p.stats, plan.stat_tiles, hidden, weight, targets, rows, width, vocab, softcap, loss, lse);
 }
 
 void launch_lmhead_loss_grad(const uint16_t* hidden, const uint16_t* weight, const int32_t* targets, const float* lse,

@@ -86,6 +86,28 @@ def test_a_large_vocabulary_in_pieces(samplers):
     check(samplers(vocab), h, w, t, 30.0)
 
 
+@pytest.mark.parametrize("rows,width,vocab,cap", [
+    (3, 64, 66000, 0.0),     # more tiles of 256 than compute units: smaller ones, the last one ragged or not
+    (70, 64, 66001, 30.0),
+    (128, 128, 90112, 3.0),
+    (100, 64, 151643, 0.0),
+    (130, 64, 66016, 0.0),
+])
+def test_a_vocabulary_of_more_tiles_than_compute_units(samplers, rows, width, vocab, cap):
+    rng = np.random.default_rng(rows + vocab)
+    h, w, t = operands(rng, rows, width, vocab, 2.0)
+    h[0] *= -4.0  # a row whose logits are large on both sides
+    dev = [v.cuda() for v in (h, w, t)]
+    loss, lse = samplers(vocab).lmhead_loss(*dev, softcap_value=cap)
+    z = ref.capped(h.double() @ w.double().T, cap)
+    want = torch.logsumexp(z, 1)
+    e = logit_error(h, w, cap)
+    assert ((lse.double().cpu() - want).abs() <= e + 2.0 ** -20 * (1 + want.abs())).all()
+    scored = (t >= 0) & (t < vocab)
+    want_loss = torch.where(scored, want - z[torch.arange(rows), torch.where(scored, t.long(), 0)], 0.0)
+    assert ((loss.double().cpu() - want_loss).abs() <= 2 * e + 2.0 ** -19 * (1 + want.abs() + want_loss.abs())).all()
+
+
 def test_the_largest_vocabulary(samplers):
     check(samplers(2097152), *operands(np.random.default_rng(27), 3, 64, 2097152, 2.0), 30.0)
 
