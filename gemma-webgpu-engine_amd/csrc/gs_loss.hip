@@ -22,8 +22,8 @@
 // kHidden and kWeight sum over an operand's rows: those tiles lie in LDS as
 // they do in memory and are transposed by the LDS reads (ds_read_b64_tr_b16).
 //
-// Few rows are bound by W's bytes (100 x 2048 x 151643: kStats 121 us for 621 MB,
-// 5.1 TB/s), many by the matrix cores: at 4096 x 2048 x 262144 kStats 3.5 ms (1.25
+// Few rows are bound by W's bytes (100 x 2048 x 151643: kStats 117 us for 621 MB,
+// 5.3 TB/s), many by the matrix cores: at 4096 x 2048 x 262144 kStats 3.5 ms (1.25
 // PFLOP/s, the cores busy for 63 %), and for a piece of 32768 vocabulary rows kGrad
 // 517 us (52 %), kHidden 400 and kWeight 403 (1.37 PFLOP/s, 69 %; a library product
 // of that size reaches 1.46). The rest is the epilogues', which one wave a SIMD has
