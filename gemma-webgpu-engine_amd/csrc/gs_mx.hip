@@ -92,7 +92,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t
 // most 2^-10 of its largest product, and the logits of random operands by 5e-6 of
 // their norm (a chain of binary32 sums: 1e-7). That is far below what the codes
 // themselves leave out (2^-4 and more of a value), and the exact alternative,
-// products of the codes widened to bf16, has a quarter of the rate and its own
+// products of the codes widened to bf16, has half the rate and its own
 // conversions.
 //
 // ---- up to 64 hidden rows: bound by W's bytes
