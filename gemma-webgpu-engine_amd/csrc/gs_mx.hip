@@ -381,14 +381,23 @@ struct WideTile {
 
 // acc += the scaled products of an e2m1 and an e4m3 operand (scales in the low
 // bytes), in place and in this order: the compiler would run the builtin's out
-// in one go, apart from the reads between them. A tile's sums are read no sooner
-// than sums_ready() after the last of these (the compiler does not count the
-// matrix core's passes through assembly).
+// in one go, apart from the reads between them. It sees no matrix instruction in
+// assembly, so neither the waits before it nor those after: kFresh, where a scale
+// has just been shifted, puts the two states between a vector instruction and the
+// product that reads its result (in front of every product they cost 2 % more at
+// 300 rows), and a tile's sums are read no sooner than sums_ready() after the last
+// of these.
+template <bool kFresh>
 __device__ __forceinline__ void add_scaled_products(f32x4& acc, const i32x4& w, const i32x8& h, int ws, int hs) {
 #ifdef __HIP_DEVICE_COMPILE__
-  asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
-               : "+a"(acc)
-               : "v"(w), "v"(h), "v"(ws), "v"(hs));
+  if constexpr (kFresh)
+    asm volatile("s_nop 1\n\tv_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
+                 : "+a"(acc)
+                 : "v"(w), "v"(h), "v"(ws), "v"(hs));
+  else
+    asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 op_sel_hi:[0,0,0] cbsz:4"
+                 : "+a"(acc)
+                 : "v"(w), "v"(h), "v"(ws), "v"(hs));
 #endif
 }
 __device__ __forceinline__ void sums_ready() {
@@ -553,8 +562,10 @@ __global__ __launch_bounds__(kWideThreads, 1) void mx_head_wide_kernel(
 #ifdef __HIP_DEVICE_COMPILE__
       __builtin_amdgcn_sched_barrier(0x6);
 #endif
-      if (a < 7) add_scaled_products(acc[a][b], w[a < 7 ? a : 0], o.h[b], ws[a < 7 ? a : 0] >> shift, hs[b]);
-      else add_scaled_products(acc[a][b], o.w7, o.h[b], o.ws7 >> shift, hs[b]);
+      const i32x4& row = a < 7 ? w[a < 7 ? a : 0] : o.w7;
+      const int scale = (a < 7 ? ws[a < 7 ? a : 0] : o.ws7) >> shift;
+      if (a == 0 || b == 0) add_scaled_products<true>(acc[a][b], row, o.h[b], scale, hs[b]);  // (the first to read a scale)
+      else add_scaled_products<false>(acc[a][b], row, o.h[b], scale, hs[b]);
 #ifdef __HIP_DEVICE_COMPILE__
       __builtin_amdgcn_sched_barrier(0x6);
 #endif
