@@ -512,7 +512,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
           }
         } else {
           const bool near = lo > -series.far && mx < series.far;  // (false with a masked row; a NaN stays one either way)
-          mx = p.cap * cap_far(mx / p.cap);                       // tanh keeps the order
+          mx = p.cap * cap_any(mx / p.cap);                       // tanh keeps the order; as near as the terms are
           const float ml = -mx * kLog2e;
           if (__all(near)) {
 #pragma unroll

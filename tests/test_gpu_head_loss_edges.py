@@ -1,0 +1,71 @@
+"""The head's cross entropy at the ends of its arguments: softcaps far from the logits' size."""
+import numpy as np
+import pytest
+import torch
+
+import head_ops as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def samplers():
+    import gsample
+
+    made = {}
+
+    def get(vocab):
+        if vocab not in made:
+            made[vocab] = gsample.Sampler(vocab_size=vocab, max_rows=1)
+        return made[vocab]
+
+    yield get
+    for s in made.values():
+        s.close()
+
+
+def operands(rng, rows, width, vocab, scale=1.0, shift=0.0):
+    """hidden, weight and targets whose logits spread by `scale` about `shift`."""
+    h = torch.from_numpy(rng.normal(0, 1, (rows, width)).astype(np.float32))
+    w = torch.from_numpy(rng.normal(0, scale * width ** -0.5, (vocab, width)).astype(np.float32))
+    h[:, 0], w[:, 0] = 1.0, shift
+    t = torch.from_numpy(rng.integers(0, vocab, rows).astype(np.int32))
+    return h.to(torch.bfloat16), w.to(torch.bfloat16), t
+
+
+# A logit's error: `width` products in binary32, a whole step each where the matrix core truncates; then the cap, whose
+# quotient, series and product are within a few steps of the capped value below 5/8 of the cap, and past it within
+# 2e-7 of the cap, itself less than twice the value: 2^-20 of the value in either case (and of the cap, 2^-21, where
+# the cap is small). The loss and lse carry the largest of the row, the exponentials' and the sum's roundings 2^-20.
+def logit_error(h, w, z):
+    return h.shape[1] * 2 * ref.U32 * (h.double().abs() @ w.double().abs().T).amax(1) + 2.0 ** -20 * z.abs().amax(1)
+
+
+def check(s, h, w, t, cap):
+    dev = [v.cuda() for v in (h, w, t)]
+    loss, lse = s.lmhead_loss(*dev, softcap_value=cap)
+    want_loss, want_lse, g, prob, scored = ref.loss(h, w, t, cap)
+    e = logit_error(h, w, ref.capped(h.double() @ w.double().T, cap))
+    assert ((lse.double().cpu() - want_lse).abs() <= e + 2.0 ** -20 * (1 + want_lse.abs())).all(), (lse, want_lse)
+    assert ((loss.double().cpu() - want_loss).abs() <= 2 * e + 2.0 ** -19 * (1 + want_lse.abs() + want_loss.abs())).all()
+    d = torch.from_numpy(np.random.default_rng(1).normal(0, 1, h.shape[0]).astype(np.float32))
+    dh, dw = s.lmhead_loss_grad(*dev, lse, d.cuda(), softcap_value=cap)
+    # g: the probability carries the logit's and lse's error, (1 - t^2) that of tanh, 2^-20 on |p - [target]|; then a
+    # rounding to bf16 (and one of dloss over the largest of them, 2^-23, among the 2^-18)
+    gd = g * d.double()[:, None]
+    pd = prob * d.double().abs()[:, None]
+    hot = torch.zeros_like(pd).scatter_(1, t.long()[:, None], d.double().abs()[:, None])
+    ge = gd.abs() * ref.U16 + pd * (2 * e + 2.0 ** -18)[:, None] + 2.0 ** -20 * (pd + hot)
+    for got, want, bound in (
+            (dh, gd @ w.double(), ge @ w.double().abs() + w.shape[0] * 2 * ref.U32 * (gd.abs() @ w.double().abs())),
+            (dw, gd.T @ h.double(), ge.T @ h.double().abs() + len(h) * 2 * ref.U32 * (gd.abs().T @ h.double().abs()))):
+        off = (got.double().cpu() - want).abs()
+        assert (off <= bound + ref.U16 * want.abs() + 1e-37).all(), float((off / (bound + ref.U16 * want.abs() + 1e-37)).max())
+
+
+@pytest.mark.parametrize("rows", [3, 70, 200])
+@pytest.mark.parametrize("cap", [1.5e3, 1e5, 1e8, 1e10, 1e20, 1e38])
+@pytest.mark.parametrize("shift", [0.0, 100.0, -120.0])
+def test_caps_far_above_the_logits(samplers, rows, cap, shift):
+    rng = np.random.default_rng(rows)
+    check(samplers(700), *operands(rng, rows, 128, 700, 3.0, shift), cap)
