@@ -551,7 +551,7 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
       lds_barrier();  // read before a fetch takes the place
     } else if constexpr (kPass == kGrad) {
       const CapSeries series(p.cap, kLog2e);
-      const float per_cap2 = 1.0f / (p.cap * kLog2e) / (p.cap * kLog2e);
+      const float per_cap2 = 1.0f / (p.cap * kLog2e) / (p.cap * kLog2e);  // (finite where the series is taken)
       // the columns' values have landed for every wave; the next tile's fetches may be under way
       asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(T::kFive ? T::kFetchB : 8 + T::kFetchB) : "memory");
       const __amdgpu_buffer_rsrc_t out = __builtin_amdgcn_make_buffer_rsrc(
@@ -575,11 +575,15 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
           }
           near = __all(most < series.far);
         }
-        if (kCap && !near) {  // (uniform) z in x's place
+        // With a cap: y = z log2(e) by the series, else (uniform) 2 z / cap, in x's place; both of its uses
+        // hold their range for any finite cap (z log2(e) over the cap's square would not).
+        const float y_log2 = near ? 1.0f : p.cap * (0.5f * kLog2e);
+        const float y_slope = near ? -per_cap2 * c.share : -0.25f * c.share;
+        if (kCap && !near) {
 #pragma unroll
           for (int a = 0; a < 8; ++a) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[a][b][e] = p.cap * kLog2e * cap_any(acc[a][b][e] / p.cap);
+            for (int e = 0; e < 4; ++e) acc[a][b][e] = 2.0f * cap_any(acc[a][b][e] / p.cap);
           }
         }
         MxU32x2 w[8];
@@ -593,10 +597,10 @@ __global__ __launch_bounds__(kLossThreads, 1) void loss_kernel(LossArgs p) {
               v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x, kLog2e, c.ll));
               slope[e] = c.share;
             } else {
-              // z log2(e), and share (1 - (z / cap)^2)
-              const float z = near ? x * series(x * x) : x;
-              v[e] = __builtin_amdgcn_exp2f(z + c.ll);
-              slope[e] = __builtin_fmaf(z * z, -per_cap2 * c.share, c.share);
+              // the probability, and share (1 - (z / cap)^2)
+              const float y = near ? x * series(x * x) : x;
+              v[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(y, y_log2, c.ll));
+              slope[e] = __builtin_fmaf(y * y, y_slope, c.share);
             }
           }
           if (any_hit) {  // (uniform)

@@ -69,3 +69,13 @@ def check(s, h, w, t, cap):
 def test_caps_far_above_the_logits(samplers, rows, cap, shift):
     rng = np.random.default_rng(rows)
     check(samplers(700), *operands(rng, rows, 128, 700, 3.0, shift), cap)
+
+
+@pytest.mark.parametrize("rows", [3, 70, 200])
+@pytest.mark.parametrize("cap", [2.0 ** -5, 1e-3, 1e-10, 1e-20, 1e-25, 1e-38, 1e-42, 3.4e38])
+def test_caps_far_below_the_logits_and_at_the_end_of_the_range(samplers, rows, cap):
+    """Below the logits most slopes are 0; a row of zeros has logits of 0, whose slope is 1 whatever the cap."""
+    rng = np.random.default_rng(rows + 1)
+    h, w, t = operands(rng, rows, 128, 700, 3.0)
+    h[1] = 0.0
+    check(samplers(700), h, w, t, cap)
