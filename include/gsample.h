@@ -399,10 +399,12 @@ int gs_lmhead_loss(gs_context* ctx, const void* hidden, const void* weight, cons
  * is not scored) from the lse that gs_lmhead_loss wrote for the same operands:
  *   g[m][v] = dloss[m] (exp(z[m][v] - lse[m]) - [v = targets[m]]) (1 - (z[m][v] / cap)^2)
  *   dhidden = g . weight (bf16 [rows][width]),  dweight = g^T . hidden (bf16 [V][width])
- * A row that is not scored adds nothing, whatever its hidden state holds. dhidden or
- * dweight may be NULL; both are 16-byte aligned. g is made again a piece of the
- * vocabulary at a time and rounded to bf16 for the two products, whose sums are in
- * binary32. No rows: dweight is zero.
+ * A row that is not scored adds nothing, whatever its hidden state holds; a dloss that
+ * is not finite reaches its own row of dhidden, and dweight. dhidden or dweight may be
+ * NULL; both are 16-byte aligned. g over the largest finite |dloss| is made again a
+ * piece of the vocabulary at a time and rounded to bf16 for the two products, whose
+ * sums are in binary32 (what lies below 2^-126 of that largest value loses bits). No
+ * rows: dweight is zero.
  * Work memory: gs_lmhead_loss, gs_lmhead_loss_grad and gs_rms_norm_grad share one
  * allocation of the context, which the largest call so far sized; it is not given
  * back before gs_destroy. Calls that take it must be ordered on one stream, and

@@ -79,3 +79,27 @@ def test_caps_far_below_the_logits_and_at_the_end_of_the_range(samplers, rows, c
     h, w, t = operands(rng, rows, 128, 700, 3.0)
     h[1] = 0.0
     check(samplers(700), h, w, t, cap)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_a_gradient_that_is_not_finite_stays_in_its_row(samplers, bad):
+    rng = np.random.default_rng(31)
+    s = samplers(700)
+    h, w, t = (v.cuda() for v in operands(rng, 150, 128, 700, 2.0))
+    t[7] = -1
+    for cap in (0.0, 20.0):
+        _, lse = s.lmhead_loss(h, w, t, softcap_value=cap)
+        d = torch.from_numpy(rng.normal(0, 1, 150).astype(np.float32)).cuda()
+        d[40], d[149] = 0.0, 0.0
+        want, _ = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=cap)
+        d[40], d[149], d[7] = bad, bad, bad
+        got, dw = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=cap)
+        alone, _ = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=cap, weight_grad=False)
+        keep = [i for i in range(150) if i not in (40, 149)]
+        for dh in (got, alone):
+            assert torch.equal(dh[keep], want[keep])
+            assert not dh[40].isfinite().any() and not dh[149].isfinite().any()
+        assert not dw.isfinite().any()  # every vocabulary row takes its share of those rows
+        d[:] = bad  # no row is finite
+        dh, _ = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=cap)
+        assert (dh[7] == 0).all() and not torch.cat([dh[:7], dh[8:]]).isfinite().any()
