@@ -717,7 +717,9 @@ __global__ __launch_bounds__(kJoinThreads) void loss_join_kernel(const float2* _
     const float l = s.x + logf(s.y);
     if (cap > 0.0f) z = cap * tanhf(z / cap);
     lse[own] = l;
-    loss[own] = scored ? l - z : 0.0f;
+    // (z's sum is in another order than the one in l: at a certain target the difference may come out below 0)
+    const float d = l - z;
+    loss[own] = !scored || d < 0.0f ? 0.0f : d;  // (a NaN stays one)
   }
 }
 

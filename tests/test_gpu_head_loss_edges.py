@@ -1,4 +1,5 @@
-"""The head's cross entropy at the ends of its arguments: softcaps far from the logits' size."""
+"""The head's cross entropy at the ends of its arguments: softcaps far from the logits' size, gradients that are not
+finite, certain targets."""
 import numpy as np
 import pytest
 import torch
@@ -103,3 +104,20 @@ def test_a_gradient_that_is_not_finite_stays_in_its_row(samplers, bad):
         d[:] = bad  # no row is finite
         dh, _ = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=cap)
         assert (dh[7] == 0).all() and not torch.cat([dh[:7], dh[8:]]).isfinite().any()
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+def test_a_certain_token_s_loss_is_never_below_zero(samplers, cap):
+    """The target's logit alone makes up the sum of exponentials, so the loss is 0 but for roundings."""
+    rng = np.random.default_rng(32)
+    h, w, t = operands(rng, 400, 704, 700, 1.0)
+    w *= 0.01
+    for m in range(400):  # row m mod 100 of W points along hidden row m
+        t[m] = m % 100
+        h[m] = h[m % 100]
+        w[m % 100] = h[m % 100] * (28.0 / 704 if cap == 0.0 else 1.0)
+    loss, lse = samplers(700).lmhead_loss(*(v.cuda() for v in (h, w, t)), softcap_value=cap)
+    want, _, _, _, _ = ref.loss(h, w, t, cap)
+    e = logit_error(h, w, ref.capped(h.double() @ w.double().T, cap))
+    assert (loss >= 0).all(), float(loss.min())
+    assert ((loss.double().cpu() - want).abs() <= 2 * e + 2.0 ** -19 * (1 + lse.double().cpu().abs())).all()
