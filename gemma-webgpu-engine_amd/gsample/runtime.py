@@ -584,9 +584,11 @@ class Sampler:
     # -- the operators on either side of the head ------------------------
     # Each takes the memory of its results (allocated when left out) and a
     # stream. With a stream it enqueues there and returns; inputs must be ready
-    # on that stream. Without one, or with 0 (the handle of torch's default
-    # stream, which the library reads as the context's own), it waits for torch's
-    # current stream, runs on the context's and waits for the results.
+    # on that stream, and results' memory that is given free to be written there
+    # (where it is left out, the stream waits for torch's current one first).
+    # Without one, or with 0 (the handle of torch's default stream, which the
+    # library reads as the context's own), it waits for torch's current stream,
+    # runs on the context's and waits for the results.
     def _tensor(self, t, name: str, dtype, shape=None):
         """The pointer of a checked contiguous tensor (None: NULL)."""
         if t is None:
@@ -622,11 +624,22 @@ class Sampler:
                                   f"not {tuple(t.shape)}")
 
     def _empty(self, shape, dtype, stream):
-        """Memory for a result of a call on `stream`: the caching allocator must
-        not hand it out again before that stream has used it."""
-        t = self.torch.empty(shape, dtype=dtype, device=self.device)
-        if stream and self.torch.cuda.current_stream(self.device).cuda_stream != stream:
-            t.record_stream(self.torch.cuda.ExternalStream(stream, device=self.device))
+        """Memory for a result of a call on `stream`. It is of torch's current stream, where work that is still
+        to come may use what the allocator handed out before: another stream waits for that work, and the
+        allocator does not hand the memory out again before that stream has used it."""
+        torch, cuda = self.torch, self.torch.cuda
+        current = cuda.current_stream(self.device) if stream else None
+        if not stream or current.cuda_stream == stream:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        other = cuda.ExternalStream(stream, device=self.device)
+        for s in (current, other):
+            with cuda.stream(s):
+                if cuda.is_current_stream_capturing():
+                    raise GSampleError(1, "a stream is under capture: give the memory of the results, or make "
+                                          "`stream` torch's current one")
+        t = torch.empty(shape, dtype=dtype, device=self.device)
+        t.record_stream(other)
+        other.wait_stream(current)
         return t
 
     def _begin(self, stream):
