@@ -776,14 +776,14 @@ class Sampler:
         sampler on it, one call; returns the rows' results."""
         b, keep = self.prepare(logits_scratch, configs, histories, forced, mask_table)
         self.mx_lmhead_sample_launch(hidden, hidden_scales, weight, weight_scales, softcap_value, logits_scratch, b)
-        self.synchronize()
         res = keep[-1].cpu().numpy().view(np.uint8).reshape(-1)[: b.rows * 16].view(RESULT_DTYPE)
         del keep
         return SampleOutput(res["token"].copy(), res["probability"].copy(), res["flags"].copy())
 
     def mx_lmhead_sample_launch(self, hidden, hidden_scales, weight, weight_scales, softcap_value: float,
                                 logits_scratch, batch: Batch, stream: Optional[int] = None):
-        """gs_mx_lmhead_sample: the 4-bit head into `logits_scratch`, then the sampler on it."""
+        """gs_mx_lmhead_sample: the 4-bit head into `logits_scratch`, then the sampler on it; the rows' results go to
+        the batch's memory (with `stream`, once that has run)."""
         ph, phs, pw, pws, m, width = self._mx_head(hidden, hidden_scales, weight, weight_scales)
         if m != batch.rows:
             raise GSampleError(1, "one hidden row per row of the batch")
@@ -791,6 +791,7 @@ class Sampler:
         s = self._begin(stream)
         self._check(self.lib.gs_mx_lmhead_sample(self.ctx, ph, phs, pw, pws, width, float(softcap_value), po,
                                                  C.byref(batch), s))
+        self._end(stream)
 
     def _loss_operands(self, hidden, weight, targets):
         torch = self.torch

@@ -114,3 +114,14 @@ def test_no_memory_across_a_capture(name, results, call, capturing):
         call(s, stream=OTHER)
     assert e.value.status == 1 and name not in s.torch.seen
     assert not any("waits" in w for w in s.torch.seen)
+
+
+@pytest.mark.parametrize("stream", [None, 0, OTHER])
+def test_head_and_sampler_without_a_stream_wait_for_the_results(stream):
+    """What the call reads may be dropped once it returns."""
+    s = sampler()
+    batch = rt.Batch()
+    batch.rows = 2
+    s.mx_lmhead_sample_launch(t(2, 64, dtype=U8), t(2, 2, dtype=U8), t(128, 32, dtype=U8), t(128, 2, dtype=U8), 0.0, t(2, 128),
+                              batch, stream=stream)
+    assert s.torch.seen == (["gs_mx_lmhead_sample"] if stream else [f"{CURRENT} drains", "gs_mx_lmhead_sample", "results"])
