@@ -16,16 +16,18 @@
 //            sums are binary32). The largest |dloss| stays out of g: where every
 //            row has the same, as in a mean, a row's largest value, at the target,
 //            is then near -1, which bf16 holds, and not a product whose rounding
-//            all rows share (dW's error at M 4096 was 1.7 times its own rounding's);
+//            all rows share (dW's error at M 4096 was 1.7 times its own rounding's;
+//            so it is 1.95e-3 of its norm, and dH's 1.94e-3, where the roundings of the
+//            results to bf16 alone make 1.66e-3);
 //   kHidden  W^T x g, summed over the piece, in shares of its vocabulary rows;
 //   kWeight  H^T x g^T, summed over the hidden rows.
 // kHidden and kWeight sum over an operand's rows: those tiles lie in LDS as
 // they do in memory and are transposed by the LDS reads (ds_read_b64_tr_b16).
 //
 // Few rows are bound by W's bytes (100 x 2048 x 151643: kStats 117 us for 621 MB,
-// 5.3 TB/s), many by the matrix cores: at 4096 x 2048 x 262144 kStats 3.5 ms (1.25
-// PFLOP/s, the cores busy for 63 %), and for a piece of 32768 vocabulary rows kGrad
-// 517 us (52 %), kHidden 400 and kWeight 403 (1.37 PFLOP/s, 69 %; a library product
+// 5.3 TB/s), many by the matrix cores: at 4096 x 2048 x 262144 kStats 3.5 ms at best (1.25
+// PFLOP/s, the cores busy for 63 %; 3.7 over a run), and for a piece of 32768 vocabulary rows kGrad
+// 529 us (52 %), kHidden 409 and kWeight 411 (1.34 PFLOP/s, 69 %; a library product
 // of that size reaches 1.46). The rest is the epilogues', which one wave a SIMD has
 // nothing to run beside; two of half the tile would read LDS twice as often.
 #include <algorithm>

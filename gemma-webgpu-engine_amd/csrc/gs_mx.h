@@ -4,9 +4,10 @@
 // magnitude) less the element format's largest exponent (2 or 8), at least
 // -127, so the largest magnitude lands in the format's top binade; what lies
 // past its largest value there (6 or 448) becomes that value, everything else
-// is rounded to nearest, ties to the even mantissa. The 8-bit and the 4-bit
-// values of a block hold relative errors of 2^-4 and 2^-2 at most above the
-// format's smallest normal value: that is the choice of the formats.
+// is rounded to nearest, ties to the even mantissa. Above the format's smallest
+// normal value a rounding is off by at most 2^-4 (8 bits) or 2^-2 (4 bits) of the
+// value; one that becomes the largest value, by up to 2^-3 (just below 512) or
+// 2^-2 (just below 8): that is the choice of the formats.
 #pragma once
 
 #include "gs_internal.h"

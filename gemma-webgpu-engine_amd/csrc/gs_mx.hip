@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kMxThreads) void mx_dequantize_kernel(const uint8_t
 // largest of them, and the groups' sums in binary32: a group of 8 is off by at
 // most 2^-10 of its largest product, and the logits of random operands by 5e-6 of
 // their norm (a chain of binary32 sums: 1e-7). That is far below what the codes
-// themselves leave out (2^-4 and more of a value), and the exact alternative,
+// themselves leave out (up to 2^-3 and 2^-2 of a value), and the exact alternative,
 // products of the codes widened to bf16, has half the rate and its own
 // conversions.
 //

@@ -292,12 +292,13 @@ void norm_backward(const NormGradArgs& a, hipStream_t s) {
 }  // namespace
 
 // Many narrow rows: a wave a row (no barrier). Few, or wide: a workgroup a row
-// (8192 rows of 2048: 28.4 us, and 30.4 with a wave a row).
+// (the forward pass of 8192 rows of 2048: 28.4 us, and 30.4 with a wave a row; the
+// gradient follows it, unmeasured the other way).
 bool norm_wave_rows(int32_t rows, int32_t width) { return rows >= 2048 && width <= 1024; }
 
 // Workgroups of the gradient's kernel: as many shares of dw. About 768, three a
-// compute unit (4099 rows of 3840: 37.7 us, with 512 41.6, with 1024 45.1), and
-// as many rows for each as can be alike.
+// compute unit of this card (4099 rows of 3840, the one size it was chosen at: 37.7 us,
+// with 512 41.6, with 1024 45.1), and as many rows for each as can be alike.
 int32_t norm_parts(int32_t rows, int32_t width) {
   const int32_t groups = norm_wave_rows(rows, width) ? rows / 4 + (rows % 4 != 0) : rows;
   const int32_t each = groups < 1152 ? 1 : groups / 768 + (groups % 768 >= 384);

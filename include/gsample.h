@@ -335,7 +335,8 @@ int gs_qat_lmhead_sample(gs_context* ctx, const float* x, int32_t width, const u
  * apart; weight [width] of weight_dtype. Written where given: summed (h), out
  * (y in dtype), and codes + scales: y in e4m3 blocks as gs_mx_quantize lays
  * them out, rounded once from binary32 (width a multiple of 32, codes 16-byte
- * aligned). width at most 16384. */
+ * aligned). width at most 16384. mean(h^2) + eps has to lie within binary32's
+ * normal numbers: where a square of h passes its range (|h| from 1.8e19 on), y is 0. */
 int gs_rms_norm(gs_context* ctx, const void* x, const void* residual, const void* weight, int32_t dtype,
                 int32_t weight_dtype, int32_t rows, int32_t width, int64_t x_stride, int64_t residual_stride,
                 float eps, float weight_offset, void* summed, void* out, uint8_t* codes, uint8_t* scales, void* stream);
@@ -374,10 +375,12 @@ int gs_mx_dequantize(gs_context* ctx, const uint8_t* codes, const uint8_t* scale
 /* The lm_head over microscaled operands: logits[m][v] = cap(hidden[m] . weight[v])
  * with hidden in e4m3 ([m_rows][width], scales [m_rows][width / 32]) and weight in
  * e2m1 ([V][width / 2], scales [V][width / 32]), both as gs_mx_quantize lays them
- * out, the cap as gs_lmhead's (softcap finite; <= 0: none). width a multiple of 64,
- * at most 16384; codes 16-byte, scales 2-byte aligned. logits f32 [m_rows][V].
+ * out, cap as in gs_lmhead but not to the bit (softcap finite; <= 0: none). width a
+ * multiple of 64, at most 16384; codes 16-byte, scales 2-byte aligned. logits f32
+ * [m_rows][V].
  * Sums are in binary32 but for the matrix instruction's own: it adds 8 neighbouring
- * products at a time, each cut 13 bits below the largest of them. */
+ * products at a time, each cut 13 bits below the largest of them. Calls of up to 64
+ * rows and of more sum in other orders: a row's logits then differ by as much. */
 int gs_mx_lmhead(gs_context* ctx, const uint8_t* hidden_codes, const uint8_t* hidden_scales,
                  const uint8_t* weight_codes, const uint8_t* weight_scales, int32_t m_rows, int32_t width,
                  float softcap, float* logits, void* stream);
@@ -388,7 +391,7 @@ int gs_mx_lmhead_sample(gs_context* ctx, const uint8_t* hidden_codes, const uint
 
 /* Softmax cross entropy of the head's logits z = cap(hidden . weight) (gs_lmhead's,
  * never written to memory): lse[m] = log(sum_v exp(z[m][v])) and
- * loss[m] = lse[m] - z[m][targets[m]], 0 where the target is outside [0, V) (a
+ * loss[m] = lse[m] - z[m][targets[m]], never below 0, 0 where the target is outside [0, V) (a
  * row that is not scored). hidden bf16 [rows][width], weight bf16 [V][width],
  * 16-byte aligned, width a multiple of 64; targets int32 [rows]; loss and lse f32
  * [rows]. width at most 65536, rows at most 2^20, rows * width below 2^30; softcap
