@@ -1,5 +1,5 @@
 """The head's cross entropy at the ends of its arguments: softcaps far from the logits' size, gradients that are not
-finite, certain targets."""
+finite, certain targets, results in place of operands."""
 import numpy as np
 import pytest
 import torch
@@ -121,3 +121,32 @@ def test_a_certain_token_s_loss_is_never_below_zero(samplers, cap):
     e = logit_error(h, w, ref.capped(h.double() @ w.double().T, cap))
     assert (loss >= 0).all(), float(loss.min())
     assert ((loss.double().cpu() - want).abs() <= 2 * e + 2.0 ** -19 * (1 + lse.double().cpu().abs())).all()
+
+
+@pytest.mark.parametrize("rows,width,vocab", [(60, 128, 700), (5000, 64, 30011)])  # (the second in pieces of the vocabulary)
+def test_gradients_in_place_of_their_operands(samplers, rows, width, vocab):
+    rng = np.random.default_rng(33)
+    s = samplers(vocab)
+    h, w, t = (v.cuda() for v in operands(rng, rows, width, vocab, 2.0))
+    t[::7] = -1
+    d = torch.from_numpy(rng.normal(0, 1, rows).astype(np.float32)).cuda()
+    _, lse = s.lmhead_loss(h, w, t, softcap_value=20.0)
+    want = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=20.0)
+    got = s.lmhead_loss_grad(h, w, t, lse, d, softcap_value=20.0, dhidden=h, dweight=w)
+    assert got[0].data_ptr() == h.data_ptr() and got[1].data_ptr() == w.data_ptr()
+    assert torch.equal(h, want[0]) and torch.equal(w, want[1])
+
+
+@pytest.mark.parametrize("rows,width", [(2500, 64), (2500, 4200), (5, 577)])
+def test_norm_gradients_in_place_of_their_inputs(samplers, rows, width):
+    rng = np.random.default_rng(34)
+    s = samplers(700)
+    for dtype in (torch.float32, torch.bfloat16):
+        of = lambda: torch.from_numpy(rng.standard_normal((rows, width), dtype=np.float32)).to(dtype).cuda()  # noqa: E731
+        h, dy, ds, w = of(), of(), of(), torch.from_numpy(rng.normal(1, 0.2, width).astype(np.float32)).cuda()
+        want, want_dw = s.rms_norm_grad(dy, h, w, dsummed=ds)
+        for place in range(3):
+            ops = [v.clone() for v in (dy, h, ds)]
+            v = w.clone()
+            s.rms_norm_grad(ops[0], ops[1], v, dsummed=ops[2], dx=ops[place], dweight=v)
+            assert torch.equal(ops[place], want) and torch.equal(v, want_dw)
