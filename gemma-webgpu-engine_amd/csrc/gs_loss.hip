@@ -57,7 +57,7 @@ typedef __attribute__((address_space(3))) i16x4* LdsTrPtr;
 struct Column {
   int32_t target;  // negative: not scored
   float ll;        // -lse log2(e)
-  float share;     // dloss over the largest |dloss|
+  float share;     // dloss over the largest finite |dloss|
   float none;
 };
 

@@ -20,6 +20,7 @@ def sampler():
 def test_a_result_s_memory_is_not_written_while_the_current_stream_uses_it(sampler):
     """A tensor that the current stream has yet to copy is dropped, and the result of a call on another stream takes
     its memory."""
+    torch.cuda.empty_cache()
     rng = np.random.default_rng(41)
     rows, width = 1500, 8000  # a size of its own, so that the allocator hands the same block out again
     x = torch.from_numpy(rng.normal(0, 1, (rows, width)).astype(np.float32)).cuda()
